@@ -27,6 +27,9 @@ GOAL_TOP_RIGHT, GOAL_LIST, GOAL_SEEDED = 0, 1, 2
 START_CENTRE, START_FIXED, START_RANDOM = 0, 1, 2
 EPS_FIXED, EPS_MULT_PER_STEP, EPS_MULT_PER_EPISODE, EPS_LINEAR = 0, 1, 2, 3
 QINIT_ZERO, QINIT_UNIFORM = 0, 1
+F32, BF16, F16 = 0, 1, 2
+MAX_TOP = 32
+ADAMW_BLOCK = 256
 
 
 class Config(C.Structure):
@@ -61,6 +64,30 @@ class Stats(C.Structure):
 
 class EvalStats(C.Structure):
     _fields_ = [("envs", C.c_int64), ("reached", C.c_int64), ("total_steps", C.c_int64), ("reward_sum", C.c_double)]
+
+
+class PolicyRows(C.Structure):
+    """cudarl_policy_rows of include/cudarl.h, field for field; pointers are device addresses (integers)."""
+    _fields_ = [("struct_size", C.c_uint32), ("type", C.c_int32), ("rows", C.c_int64), ("actions", C.c_int64), ("logits", C.c_void_p), ("row_stride", C.c_int64),
+                ("legal", C.c_void_p), ("legal_stride", C.c_int64), ("taken", C.c_void_p), ("inv_temperature", C.c_float), ("reserved0", C.c_int32)]
+
+    def __init__(self, logits, type, rows, actions, row_stride=None, legal=None, legal_stride=0, taken=None, inv_temperature=1.0):
+        super().__init__(C.sizeof(PolicyRows), type, rows, actions, logits, actions if row_stride is None else row_stride, legal, legal_stride, taken, inv_temperature, 0)
+
+
+class AdamWTensor(C.Structure):
+    """cudarl_adamw_tensor of include/cudarl.h, field for field; pointers are device addresses (integers)."""
+    _fields_ = [("count", C.c_int64), ("param", C.c_void_p), ("grad", C.c_void_p), ("master", C.c_void_p), ("moment1", C.c_void_p), ("moment2", C.c_void_p),
+                ("scale1", C.c_void_p), ("scale2", C.c_void_p), ("param_type", C.c_int32), ("grad_type", C.c_int32), ("lr_scale", C.c_float), ("weight_decay", C.c_float)]
+
+
+class AdamWConfig(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("device", C.c_int32), ("state_bits", C.c_int32), ("max_grad_norm", C.c_float),
+                ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("seed", C.c_uint64), ("step", C.c_int64)]
+
+
+class AdamWStats(C.Structure):
+    _fields_ = [("step", C.c_int64), ("skipped", C.c_int64), ("grad_norm", C.c_double)]
 
 
 # every exported symbol of include/cudarl.h with (restype, argtypes)
@@ -106,6 +133,13 @@ ABI = {
     "cudarl_kernel_timing": (C.c_int, [_P, C.c_int]),
     "cudarl_kernel_time_ms": (C.c_int, [_P, C.POINTER(C.c_float), C.POINTER(C.c_int64)]),
     "cudarl_debug_set_copy_wait_polls": (C.c_int, [_P, C.c_int32]),
+    "cudarl_policy_logprobs": (C.c_int, [C.POINTER(PolicyRows), _P, _P, _P, C.c_int32, _P, _P, _P]),
+    "cudarl_policy_logprobs_backward": (C.c_int, [C.POINTER(PolicyRows), _P, _P, _P, _P, C.c_int64, _P]),
+    "cudarl_adamw_create": (C.c_int, [C.POINTER(AdamWConfig), C.c_int32, C.POINTER(AdamWTensor), C.POINTER(_P)]),
+    "cudarl_adamw_destroy": (None, [_P]),
+    "cudarl_adamw_step": (C.c_int, [_P, C.c_float, C.c_float, _P]),
+    "cudarl_adamw_set_gradients": (C.c_int, [_P, C.POINTER(_P), _P]),
+    "cudarl_adamw_get_stats": (C.c_int, [_P, C.POINTER(AdamWStats)]),
     "cudarl_version": (C.c_char_p, []),
 }
 
@@ -378,3 +412,60 @@ def comm_unique_id():
     if rc != 0:
         raise CudarlError(rc, load().cudarl_last_global_error().decode())
     return buf.raw
+
+
+def _global_ck(rc):
+    if rc != 0:
+        raise CudarlError(rc, load().cudarl_last_global_error().decode())
+
+
+def policy_logprobs(rows, logprob=None, entropy=None, stats=None, top=0, top_actions=None, top_logprobs=None, stream=None):
+    """cudarl_policy_logprobs: log probability of the actions taken, entropy and the most probable actions of PolicyRows.  Outputs are device addresses
+    (what a tensor's data_ptr() gives), `stream` a cudaStream_t as an integer."""
+    rc = load().cudarl_policy_logprobs(rows, logprob, entropy, stats, top, top_actions, top_logprobs, stream)
+    if rc != 0:
+        _global_ck(rc)
+
+
+def policy_logprobs_backward(rows, stats, grad_logprob, grad_entropy, grad_logits, grad_stride=None, stream=None):
+    """cudarl_policy_logprobs_backward: the gradient of the logits, with the `stats` that policy_logprobs wrote for the same rows."""
+    rc = load().cudarl_policy_logprobs_backward(rows, stats, grad_logprob, grad_entropy, grad_logits, rows.actions if grad_stride is None else grad_stride, stream)
+    if rc != 0:
+        _global_ck(rc)
+
+
+class AdamW:
+    """AdamW over all tensors of a network, one call a step, through the C ABI.  `tensors`: a list of AdamWTensor; their memory stays the caller's."""
+
+    def __init__(self, tensors, state_bits=32, beta1=0.9, beta2=0.999, eps=1e-8, max_grad_norm=0.0, seed=0, step=0, device=0):
+        self.h = C.c_void_p()
+        self.lib = load()
+        self.count = len(tensors)
+        cfg = AdamWConfig(C.sizeof(AdamWConfig), device, state_bits, max_grad_norm, beta1, beta2, eps, seed, step)
+        _global_ck(self.lib.cudarl_adamw_create(C.byref(cfg), self.count, (AdamWTensor * max(1, self.count))(*tensors), C.byref(self.h)))
+
+    def close(self):
+        if self.h:
+            self.lib.cudarl_adamw_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def step(self, lr, grad_scale=1.0, stream=None):
+        rc = self.lib.cudarl_adamw_step(self.h, lr, grad_scale, stream)
+        if rc != 0:
+            _global_ck(rc)
+
+    def set_gradients(self, grads, stream=None):
+        if len(grads) != self.count:
+            raise ValueError("%d gradients for %d tensors" % (len(grads), self.count))
+        _global_ck(self.lib.cudarl_adamw_set_gradients(self.h, (_P * max(1, self.count))(*grads), stream))
+
+    def get_stats(self):
+        s = AdamWStats()
+        _global_ck(self.lib.cudarl_adamw_get_stats(self.h, C.byref(s)))
+        return s

@@ -861,6 +861,11 @@ void free_all(cudarl_ctx* c) {
 }  // namespace
 
 // =================================================================================================
+int cudarl::fail_global(int code, const char* text) noexcept {
+    try { g_err = text; } catch (...) {}
+    return code;
+}
+
 extern "C" {
 
 const char* cudarl_version(void) { return "0.1.0"; }

@@ -10,4 +10,7 @@ struct SingleStep { int32_t x, y; float reward; bool done; };
 int step_single_begin(cudarl_ctx* ctx, bool reset, int32_t action);
 int step_single_end(cudarl_ctx* ctx, SingleStep* out);
 
+// Sets the text of cudarl_last_global_error and gives `code` back.
+int fail_global(int code, const char* text) noexcept;
+
 }  // namespace cudarl

@@ -224,6 +224,107 @@ int cudarl_add_trap(cudarl_ctx* ctx, int32_t x, int32_t y, float penalty);
  * receives how many there are.  cells / penalties may be NULL. */
 int cudarl_get_traps(cudarl_ctx* ctx, int32_t capacity, int32_t* cells, float* penalties, int32_t* count);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * A learned policy (no counterpart in the reference, whose only policy is the table).  cudarl_step_actions_device takes its
+ * actions from a policy of the caller's own; these calls are what training that policy needs besides its network: the log
+ * probability of the actions taken with the entropy and the most probable alternatives, their gradient with respect to the
+ * logits, and the AdamW step of the network's tensors.  As in cudarl_update_batch_static all arrays are DEVICE pointers owned
+ * by the caller, the work is asynchronous on `stream` (a cudaStream_t, NULL = default stream), a bad argument returns a
+ * negative code and launches nothing; cudarl_last_global_error has a text.  The calls run on the device that the arrays are
+ * on, whichever is current; the stream has to be one of that device's.  They may be captured into a CUDA graph. */
+enum { CUDARL_F32 = 0, CUDARL_BF16 = 1, CUDARL_F16 = 2 };
+#define CUDARL_MAX_TOP 32
+
+/* Rows of logits.  Row r, action a is logits[r*row_stride + a], of the type given, at any alignment that the type has; the log
+ * probabilities are those of the distribution softmax(inv_temperature * logits) over the legal actions.  An action whose mask
+ * byte is 0 does not exist, whatever its logit holds; a logit of minus infinity has probability 0. */
+typedef struct cudarl_policy_rows {
+    uint32_t struct_size;   /* = sizeof(cudarl_policy_rows); checked */
+    int32_t  type;          /* CUDARL_F32, CUDARL_BF16 or CUDARL_F16 */
+    int64_t  rows;
+    int64_t  actions;       /* of a row: 1 .. 2^31 - 1 */
+    const void* logits;
+    int64_t  row_stride;    /* in values, >= actions */
+    const uint8_t* legal;   /* NULL = all are; else legal[r*legal_stride + a], 0 = illegal */
+    int64_t  legal_stride;  /* >= actions, or 0 = one mask for all rows */
+    const int32_t* taken;   /* the action taken in each row; one outside 0 .. actions-1 (padding, say -1) is no action: its log
+                               probability is given as 0 and has no gradient.  NULL = none were taken */
+    float    inv_temperature; /* finite, > 0 */
+    int32_t  reserved0;
+} cudarl_policy_rows;
+
+/* logprob[rows]: of the action taken.  entropy[rows]: in nats.  stats[4*rows], 16-byte aligned: what the backward call reads.
+ * top_actions / top_logprobs [rows*top]: the `top` (0 .. CUDARL_MAX_TOP) most probable actions in falling order, of equal
+ * logits the lowest action first; places that no action is left for hold -1 and minus infinity.  Any output may be NULL (the
+ * two top arrays only together with top = 0).
+ * A row in which nothing has any probability (no legal action, or minus infinity in every one): log probability minus
+ * infinity, entropy 0.  A row that holds a NaN or plus infinity among its legal logits: NaN, and -1 for its alternatives.
+ * Two logits whose difference passes a float's range are infinitely far apart.
+ * Sums are held in 32 bits; results do not depend on anything but the row and, in their last bits, on how many there are. */
+int cudarl_policy_logprobs(const cudarl_policy_rows* p, float* logprob, float* entropy, float* stats,
+                           int32_t top, int32_t* top_actions, float* top_logprobs, void* stream);
+/* grad_logits[r*grad_stride + a] (of the logits' type) = what grad_logprob[rows] and grad_entropy[rows] (either may be NULL =
+ * zeros) make of the gradient of the logits; with the same rows and the `stats` of the call above.  Illegal actions and rows
+ * without any probability get 0.  grad_logits may be the logits themselves (same pointer and stride): they are then
+ * replaced; any other overlap is the caller's mistake.  Nothing is written between the rows. */
+int cudarl_policy_logprobs_backward(const cudarl_policy_rows* p, const float* stats, const float* grad_logprob,
+                                    const float* grad_entropy, void* grad_logits, int64_t grad_stride, void* stream);
+
+/* AdamW with decoupled weight decay over all tensors of a network at once:
+ *   g' = g * grad_scale * clip          m' = beta1 m + (1 - beta1) g'        v' = beta2 v + (1 - beta2) g'^2
+ *   w' = w - lr lr_scale (weight_decay w + (m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps))
+ * in 32 bits, rounded once to the weights' type (t = 1 for the first step).  With a master the step is that of the master and
+ * `param` receives a copy rounded to its type.
+ * With state_bits = 32 the moments m and v are floats.  With 8, moment1 holds m and moment2 the root of v as e4m3 codes, each
+ * block of 256 consecutive values (the last may be shorter) times its scale: the block's largest magnitude / 448.  A code is
+ * rounded up or down by 16 random bits of the Philox stream of (seed, step, place), so that small changes are not lost on
+ * average; a root above zero never becomes 0.  The step itself uses the moments before they are rounded.  Moments (and scales)
+ * that are all zero are the start.
+ * With max_grad_norm > 0: clip = min(1, max_grad_norm / (norm + 1e-6)) with the norm of grad_scale * g over all tensors (sums
+ * in 64 bits, always in the same order); a norm that is infinite or NaN makes the step change nothing, and it is counted as
+ * skipped. */
+#define CUDARL_ADAMW_BLOCK 256
+typedef struct cudarl_adamw_tensor {
+    int64_t     count;       /* values, 0 allowed */
+    void*       param;
+    const void* grad;        /* may be NULL until cudarl_adamw_set_gradients */
+    float*      master;      /* NULL: param is the only copy of the weights */
+    void*       moment1;     /* count floats, or count bytes */
+    void*       moment2;
+    float*      scale1;      /* 8 bits only: (count + 255) / 256 floats */
+    float*      scale2;
+    int32_t     param_type, grad_type; /* CUDARL_F32, CUDARL_BF16 or CUDARL_F16 */
+    float       lr_scale, weight_decay; /* finite, >= 0 */
+} cudarl_adamw_tensor;
+typedef struct cudarl_adamw_config {
+    uint32_t struct_size;    /* = sizeof(cudarl_adamw_config); checked */
+    int32_t  device;         /* the device that every tensor is on */
+    int32_t  state_bits;     /* 32 or 8 */
+    float    max_grad_norm;  /* 0 = no clipping */
+    double   beta1, beta2, eps; /* 0 <= beta < 1, 1e-30 <= eps <= 1e30; in double, because 1 - beta2 has few of a float's digits */
+    uint64_t seed;           /* of the rounding of 8-bit moments */
+    int64_t  step;           /* steps already taken (a resumed run), >= 0 */
+} cudarl_adamw_config;
+typedef struct cudarl_adamw_stats {
+    int64_t step;            /* steps taken, the resumed run's included */
+    int64_t skipped;         /* steps that a norm which was no finite number kept from happening */
+    double  grad_norm;       /* of the last step with clipping: before clipping, grad_scale included */
+} cudarl_adamw_stats;
+typedef struct cudarl_adamw cudarl_adamw;
+
+/* The handle keeps the list of the tensors and the step count on the device; the tensors' memory stays the caller's and has
+ * to outlive it.  Tensors must not overlap.  One handle's calls are ordered by the caller (one stream, or events). */
+int  cudarl_adamw_create(const cudarl_adamw_config* cfg, int32_t count, const cudarl_adamw_tensor* tensors, cudarl_adamw** out);
+/* Waits for the device. */
+void cudarl_adamw_destroy(cudarl_adamw* opt);
+/* One step of all tensors.  The step count is on the device: a captured graph counts on with every replay (lr and grad_scale
+ * stay those of the capture). */
+int  cudarl_adamw_step(cudarl_adamw* opt, float lr, float grad_scale, void* stream);
+/* New gradient pointers for the tensors in order (host array of `count` device pointers); not while `stream` is captured. */
+int  cudarl_adamw_set_gradients(cudarl_adamw* opt, const void* const* grads, void* stream);
+/* Waits for the device. */
+int  cudarl_adamw_get_stats(cudarl_adamw* opt, cudarl_adamw_stats* out);
+
 /* Switch the max(0, .) clamp of the flat reference kernel (src/kernels.cu:102-110) on or off. */
 int cudarl_set_legacy_clamp(cudarl_ctx* ctx, int on);
 
