@@ -64,6 +64,13 @@ public:
     ~CurrentDevice() { if (before_ >= 0) cudaSetDevice(before_); }
 };
 
+// Of the current device.
+inline cudaError_t multiprocessors(int* out) noexcept {
+    int device = 0;
+    const cudaError_t e = cudaGetDevice(&device);
+    return e != cudaSuccess ? e : cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, device);
+}
+
 // One value as a float, and a float rounded to nearest into one.
 template <int TYPE> struct Of;
 template <> struct Of<CUDARL_F32> {

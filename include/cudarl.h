@@ -234,6 +234,7 @@ int cudarl_get_traps(cudarl_ctx* ctx, int32_t capacity, int32_t* cells, float* p
  * on, whichever is current; the stream has to be one of that device's.  They may be captured into a CUDA graph. */
 enum { CUDARL_F32 = 0, CUDARL_BF16 = 1, CUDARL_F16 = 2 };
 #define CUDARL_MAX_TOP 32
+#define CUDARL_MAX_POLICY_ACTIONS (1 << 30)
 
 /* Rows of logits.  Row r, action a is logits[r*row_stride + a], of the type given, at any alignment that the type has; the log
  * probabilities are those of the distribution softmax(inv_temperature * logits) over the legal actions.  An action whose mask
@@ -242,14 +243,14 @@ typedef struct cudarl_policy_rows {
     uint32_t struct_size;   /* = sizeof(cudarl_policy_rows); checked */
     int32_t  type;          /* CUDARL_F32, CUDARL_BF16 or CUDARL_F16 */
     int64_t  rows;
-    int64_t  actions;       /* of a row: 1 .. 2^31 - 1 */
+    int64_t  actions;       /* of a row: 1 .. CUDARL_MAX_POLICY_ACTIONS */
     const void* logits;
     int64_t  row_stride;    /* in values, >= actions */
     const uint8_t* legal;   /* NULL = all are; else legal[r*legal_stride + a], 0 = illegal */
     int64_t  legal_stride;  /* >= actions, or 0 = one mask for all rows */
     const int32_t* taken;   /* the action taken in each row; one outside 0 .. actions-1 (padding, say -1) is no action: its log
                                probability is given as 0 and has no gradient.  NULL = none were taken */
-    float    inv_temperature; /* finite, > 0 */
+    float    inv_temperature; /* 1e-6 .. 1e6 */
     int32_t  reserved0;
 } cudarl_policy_rows;
 
