@@ -1,11 +1,13 @@
 // adamw.cu -- one AdamW step over all tensors of a network, moments in 32 bits or in 8, with clipping by the global norm.
 //
-// The handle keeps on the device: the list of the tensors, a list of the pieces of them that one warp takes at a time (256 values, the block of one
-// scale of the 8-bit moments), and the step count with what depends on it.  Nothing of a step comes from the host but lr and grad_scale, so a
+// The handle keeps on the device: the list of the tensors, a list of the pieces of them that a block of threads takes at a time (up to eight blocks of 256 values,
+// a block being what one scale of the 8-bit moments is for), and the step count with what depends on it.  Nothing of a step comes from the host but lr and grad_scale, so a
 // captured step counts on.
+#include "async_copy.cuh"
 #include "caller_arrays.cuh"
 #include "rules.cuh"
 #include <cuda_fp8.h>
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -16,35 +18,109 @@ using namespace cudarl;
 
 constexpr unsigned TAG_OPTIMIZER = 0x4F50544Du;
 constexpr int BLOCK = CUDARL_ADAMW_BLOCK;
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int WARPS = 8, THREADS = 32 * (WARPS + 1);     // eight warps that compute, and one that has their next pieces copied
+constexpr int RESIDENT = 3;                    // blocks of threads on an SM
 
-struct Tensor {
+struct alignas(16) Tensor {
     void* param; const void* grad; float* master; void* moment1; void* moment2; float* scale1; float* scale2;
     long long count;
-    int param_type, grad_type;
     float lr_scale, decay;
+    unsigned char param_type, grad_type;
+    unsigned char wide;                       // every array but the gradient begins at an address that bulk copies can start at and eight values can be stored to at once
+    unsigned char wide_grad;                  // the gradient does
+    unsigned reserved;
 };
-struct Piece { unsigned tensor, block; };     // the tensor's values block * 256 ...
+struct Piece { unsigned tensor, block, blocks, number; };   // `blocks` blocks (1 .. WARPS) of a tensor from its block `block` on, which is number `number` of all
 
 struct Control {
     long long step, skipped;
-    double norm, power1, power2;              // powers of the betas for the step to come
+    double norm, power1, power2;              // powers of the betas for the step to come ...
+    float fix1, root_fix2;                    // ... and what they make of it: 1 / (1 - power1), and the root of 1 / (1 - power2)
     float clip;
     unsigned go;                              // 0: the norm was no finite number
     unsigned done, done_norm;                 // blocks of the launch that have finished
+    unsigned error;                           // CUDARL_DEVERR_*
 };
 
-struct Settings { float beta1, rest1, beta2, rest2, eps; unsigned k0, k1; int clipped; double power1, power2; };   // rest = 1 - beta
+struct Settings {
+    float beta1, rest1, beta2, rest2, eps;    // rest = 1 - beta
+    unsigned keys[20];                        // of the ten Philox rounds
+    int clipped;
+    double power1, power2;                    // the betas
+};
 
-__device__ __forceinline__ float load(const void* p, int type, long long i) {
-    if (type == CUDARL_F32) return static_cast<const float*>(p)[i];
-    if (type == CUDARL_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    return __half2float(static_cast<const __half*>(p)[i]);
+// Eight values from `i` on as they lie there: one access of 16 or 32 bytes where `wide`, else one by one up to `len` (zeros behind that).  They are made
+// floats of in a call of its own, so that a thread has all its loads on their way before it waits for the first.
+struct Raw { unsigned v[8]; };
+__device__ __forceinline__ void load8(Raw& r, const void* p, int type, long long i, bool wide, int len) {
+    if (type == CUDARL_F32) {
+        const unsigned* at = static_cast<const unsigned*>(p) + i;
+        if (wide) asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7]) : "l"(at));
+        else
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r.v[k] = k < len ? at[k] : 0u;
+    } else {
+        const unsigned short* at = static_cast<const unsigned short*>(p) + i;
+        if (wide) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "l"(at));
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r.v[k] = (2 * k < len ? at[2 * k] : 0u) | (2 * k + 1 < len ? (unsigned)at[2 * k + 1] << 16 : 0u);
+    }
 }
-__device__ __forceinline__ void store(void* p, int type, long long i, float v) {
-    if (type == CUDARL_F32) static_cast<float*>(p)[i] = v;
-    else if (type == CUDARL_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+__device__ __forceinline__ void floats8(const Raw& r, int type, float (&x)[8]) {
+    if (type == CUDARL_F32)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(r.v[k]);
+    else if (type == CUDARL_BF16)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { x[2 * k] = __uint_as_float(r.v[k] << 16); x[2 * k + 1] = __uint_as_float(r.v[k] & 0xFFFF0000u); }
+    else
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.v[k])); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
+}
+__device__ __forceinline__ void store8(void* p, int type, long long i, bool wide, int len, const float (&x)[8]) {
+    if (type == CUDARL_F32) {
+        float* at = static_cast<float*>(p) + i;
+        if (wide) asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" :: "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]), "l"(at) : "memory");
+        else
+#pragma unroll
+            for (int k = 0; k < 8; ++k) if (k < len) at[k] = x[k];
+        return;
+    }
+    unsigned v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (type == CUDARL_BF16) { const __nv_bfloat162 w = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]); v[k] = *reinterpret_cast<const unsigned*>(&w); }
+        else { const __half2 w = __floats2half2_rn(x[2 * k], x[2 * k + 1]); v[k] = *reinterpret_cast<const unsigned*>(&w); }
+    }
+    if (wide) *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p) + i) = make_uint4(v[0], v[1], v[2], v[3]);
+    else {
+        unsigned short* at = static_cast<unsigned short*>(p) + i;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) if (k < len) at[k] = (unsigned short)(v[k / 2] >> (k % 2 ? 16 : 0));
+    }
+}
+__device__ __forceinline__ uint2 load_codes(const void* p, long long i, bool wide, int len) {
+    const unsigned char* at = static_cast<const unsigned char*>(p) + i;
+    if (wide) return *reinterpret_cast<const uint2*>(at);
+    unsigned v[2] = {0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (k < len) v[k / 4] |= (unsigned)at[k] << (8 * (k % 4));
+    return make_uint2(v[0], v[1]);
+}
+__device__ __forceinline__ void store_codes(void* p, long long i, bool wide, int len, uint2 c) {
+    unsigned char* at = static_cast<unsigned char*>(p) + i;
+    if (wide) { *reinterpret_cast<uint2*>(at) = c; return; }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (k < len) at[k] = (unsigned char)((k < 4 ? c.x : c.y) >> (8 * (k % 4)));
+}
+__device__ __forceinline__ void from_codes(unsigned v, float* x) {           // four codes
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> (16 * k)), __NV_E4M3));
+        const float2 f = __half22float2(h);
+        x[2 * k] = f.x; x[2 * k + 1] = f.y;
+    }
 }
 
 __device__ __forceinline__ bool last_block(unsigned* done) {
@@ -57,120 +133,352 @@ __device__ __forceinline__ bool last_block(unsigned* done) {
     return true;
 }
 
+// ------------------------------------------------------------------------------------------------ pieces on their way to shared memory
+// A piece's arrays as they lie in memory: what is whole blocks of aligned arrays comes by bulk copies, several pieces ahead of the warps that compute; the last,
+// shorter block of a tensor, and arrays that are not aligned, those warps load themselves.  Without the copies ahead all warps of the GPU load, then compute, at
+// the same time: with moments of 8 bits, whose arithmetic takes as long as their memory traffic, the two times then add up.
+template <int BITS> struct Stage {                                           // BITS = 0: the gradients alone
+    unsigned char g[WARPS * BLOCK * 4];
+    unsigned char w[BITS ? WARPS * BLOCK * 4 : 16];
+    unsigned char m[BITS == 32 ? WARPS * BLOCK * 4 : BITS == 8 ? WARPS * BLOCK : 16], v[BITS == 32 ? WARPS * BLOCK * 4 : BITS == 8 ? WARPS * BLOCK : 16];
+    float scale1[WARPS], scale2[WARPS];
+    Tensor tensor;
+    Piece piece;
+};
+template <int BITS> struct Ring {
+    static constexpr int STAGES = BITS == 32 ? 2 : 3;
+    Stage<BITS> stage[STAGES];
+    unsigned long long full[STAGES], empty[STAGES];
+};
+static_assert(sizeof(Tensor) % 16 == 0 && sizeof(Piece) % 16 == 0 && sizeof(Ring<8>) % 16 == 0 && sizeof(Stage<8>) % 16 == 0 && sizeof(Stage<32>) % 16 == 0 && sizeof(Stage<0>) % 16 == 0,
+              "bulk copies take multiples of 16 bytes");
+__device__ __forceinline__ void copy4(void* to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(to)), "l"(from) : "memory"); }
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory"); }
+
+// Of a piece: how many of its blocks come by copies.
+template <int BITS> __device__ __forceinline__ unsigned copied_blocks(const Tensor& t, const Piece& pc) {
+    const long long whole = t.count / BLOCK - pc.block;
+    if (!t.wide_grad || (BITS && !t.wide)) return 0u;
+    return whole < (long long)pc.blocks ? (unsigned)max(whole, 0ll) : pc.blocks;
+}
+
+template <int BITS> __device__ void init_ring(Ring<BITS>& ring) {
+    if (threadIdx.x == 0u)
+        for (int i = 0; i < Ring<BITS>::STAGES; ++i) { mbar_init(&ring.full[i], BITS == 8 ? 33u : 1u); mbar_init(&ring.empty[i], WARPS); }
+    __syncthreads();
+}
+
+// The copying warp.  Its lanes look up 32 pieces at a time, then each has its own copied when its turn and a stage come.
+template <int BITS> __device__ void copy_pieces(Ring<BITS>& ring, const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl) {
+    const unsigned lane = threadIdx.x % 32u;
+    unsigned at = 0u, parity = 1u;                                           // the stage that is next, and which phase of `empty` lets it be filled
+    bool fine = true;
+    for (unsigned long long base = blockIdx.x; base < n && fine; base += 32ull * gridDim.x) {
+        const unsigned long long k = base + (unsigned long long)lane * gridDim.x;
+        const Piece pc = k < n ? pieces[k] : Piece{0u, 0u, 0u, 0u};
+        const Tensor t = k < n ? tensors[pc.tensor] : Tensor{};
+        for (unsigned turn = 0; turn < 32u && base + (unsigned long long)turn * gridDim.x < n && fine; ++turn) {
+            Stage<BITS>& st = ring.stage[at];
+            unsigned long long* const bar = &ring.full[at];
+            if (lane == turn) fine = mbar_wait(&ring.empty[at], parity, 0u);
+            fine = __shfl_sync(~0u, fine, turn);
+            if (!fine) break;
+            if (BITS == 8) {                                                 // the scales of its blocks lie anywhere: a lane copies each
+                const float* const scale1 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(t.scale1 + pc.block), turn));
+                const float* const scale2 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(t.scale2 + pc.block), turn));
+                const unsigned blocks = __shfl_sync(~0u, pc.blocks, turn), which = lane % WARPS;
+                if (lane < 2u * WARPS && which < blocks) copy4(lane < WARPS ? &st.scale1[which] : &st.scale2[which], (lane < WARPS ? scale1 : scale2) + which);
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+            }
+            if (lane == turn) {
+                const unsigned values = copied_blocks<BITS>(t, pc) * BLOCK;
+                const long long first = (long long)pc.block * BLOCK;
+                const unsigned of_g = t.grad_type == CUDARL_F32 ? 4u : 2u, of_w = t.master || t.param_type == CUDARL_F32 ? 4u : 2u, of_m = BITS == 32 ? 4u : 1u;
+                mbar_arrive_expect_tx(bar, (unsigned)(sizeof(Tensor) + sizeof(Piece)) + values * (of_g + (BITS ? of_w + 2u * of_m : 0u)));
+                bulk_g2s(&st.tensor, tensors + pc.tensor, sizeof(Tensor), bar);
+                bulk_g2s(&st.piece, pieces + k, sizeof(Piece), bar);
+                if (values) {
+                    bulk_g2s(st.g, static_cast<const char*>(t.grad) + first * of_g, values * of_g, bar);
+                    if (BITS) {
+                        bulk_g2s(st.w, (t.master ? reinterpret_cast<const char*>(t.master) : static_cast<const char*>(t.param)) + first * of_w, values * of_w, bar);
+                        bulk_g2s(st.m, static_cast<const char*>(t.moment1) + first * of_m, values * of_m, bar);
+                        bulk_g2s(st.v, static_cast<const char*>(t.moment2) + first * of_m, values * of_m, bar);
+                    }
+                }
+            }
+            __syncwarp();
+            if (++at == Ring<BITS>::STAGES) { at = 0u; parity ^= 1u; }
+        }
+    }
+    if (!fine) {                                                             // given up: nothing may still be under way when the block ends
+        if (lane == 0u) {
+            atomicOr(&ctl->error, ERR_COPY_TIMEOUT);
+            for (int i = 0; i < Ring<BITS>::STAGES; ++i) { (void)mbar_wait(&ring.full[i], 0u, 1u << 16); (void)mbar_wait(&ring.full[i], 1u, 1u << 16); }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+    }
+}
+
+// Eight values of a block in a stage: 32 or 16 bytes a lane.
+__device__ __forceinline__ void unstage8(Raw& r, const unsigned char* from, int type, unsigned warp, unsigned lane) {
+    if (type == CUDARL_F32) {
+        const uint4* at = reinterpret_cast<const uint4*>(from) + (warp * 32u + lane) * 2u;
+        const uint4 a = at[0], b = at[1];
+        r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w; r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
+    } else {
+        const uint4 a = reinterpret_cast<const uint4*>(from)[warp * 32u + lane];
+        r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
+    }
+}
+
+// The sum of the computing warps' values in thread 0, always in the same order.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double warp_sum[WARPS];
+    for (int by = 16; by; by /= 2) v += __shfl_xor_sync(~0u, v, by);
+    __syncthreads();
+    if (threadIdx.x % 32u == 0u && threadIdx.x / 32u < WARPS) warp_sum[threadIdx.x / 32u] = v;
+    __syncthreads();
+    v = warp_sum[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) v += warp_sum[w];
+    return v;
+}
+
 // Sum of squares of all gradients, in 64 bits and in an order that only the list of pieces and the grid make; the last block adds the blocks' sums.
-__global__ void __launch_bounds__(THREADS) k_grad_norm(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) k_grad_norm(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
+    asm volatile("griddepcontrol.launch_dependents;");                       // the step's blocks may come as these go: they load before they wait for the norm
+    extern __shared__ __align__(128) unsigned char shared_bytes[];
+    Ring<0>& ring = *reinterpret_cast<Ring<0>*>(shared_bytes);
+    init_ring(ring);
     double sum = 0.0;
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
-    for (unsigned k = blockIdx.x * WARPS + warp; k < n; k += gridDim.x * WARPS) {
-        const Piece pc = pieces[k];
-        const Tensor& t = tensors[pc.tensor];
-        const long long from = (long long)pc.block * BLOCK;
-        const int len = (int)min((long long)BLOCK, t.count - from);
-        for (int i = lane; i < len; i += 32) { const double g = load(t.grad, t.grad_type, from + i); sum += g * g; }
+    if (warp == WARPS) copy_pieces(ring, tensors, pieces, n, ctl);
+    else {
+        unsigned at = 0u, parity = 0u;
+        for (unsigned long long k = blockIdx.x; k < n; k += gridDim.x) {
+            Stage<0>& st = ring.stage[at];
+            if (!mbar_wait(&ring.full[at], parity, 0u)) { if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT); break; }
+            const Piece pc = st.piece;
+            const int type = st.tensor.grad_type;
+            Raw raw;
+            const bool mine = warp < pc.blocks;
+            if (mine) {
+                if (warp < copied_blocks<0>(st.tensor, pc)) unstage8(raw, st.g, type, warp, lane);
+                else {
+                    const long long from = (long long)(pc.block + warp) * BLOCK + lane * 8u;
+                    load8(raw, st.tensor.grad, type, from, false, (int)min(8ll, st.tensor.count - from));
+                }
+            }
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(&ring.empty[at]);
+            if (++at == Ring<0>::STAGES) { at = 0u; parity ^= 1u; }
+            if (!mine) continue;
+            float g[8];
+            floats8(raw, type, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+        }
     }
-    __shared__ double shared[THREADS];
-    shared[threadIdx.x] = sum;
-    __syncthreads();
-    for (unsigned o = THREADS / 2; o; o >>= 1) {
-        if (threadIdx.x < o) shared[threadIdx.x] += shared[threadIdx.x + o];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) part[blockIdx.x] = shared[0];
+    sum = block_sum(sum);
     __shared__ bool last;
-    const bool l = last_block(&ctl->done_norm);
-    if (threadIdx.x == 0) last = l;
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = sum;
+        __threadfence();
+        last = atomicAdd(&ctl->done_norm, 1u) + 1u == gridDim.x;
+        __threadfence();
+    }
     __syncthreads();
     if (!last) return;
     sum = 0.0;
-    for (unsigned b = threadIdx.x; b < gridDim.x; b += THREADS) sum += __ldcg(part + b);
-    shared[threadIdx.x] = sum;
-    __syncthreads();
-    for (unsigned o = THREADS / 2; o; o >>= 1) {
-        if (threadIdx.x < o) shared[threadIdx.x] += shared[threadIdx.x + o];
-        __syncthreads();
-    }
+    if (threadIdx.x < 32u * WARPS)
+        for (unsigned b = threadIdx.x; b < gridDim.x; b += 32u * WARPS) sum += __ldcg(part + b);
+    sum = block_sum(sum);
     if (threadIdx.x == 0) {
-        const double norm = sqrt(shared[0]) * fabs((double)grad_scale);
+        const double norm = sqrt(sum) * fabs((double)grad_scale);
+        ctl->done_norm = 0u;
         ctl->norm = norm;
         ctl->go = isfinite(norm) ? 1u : 0u;
         ctl->clip = (float)fmin(1.0, (double)max_norm / (norm + 1e-6));
     }
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-    return v;
-}
-
 // |y| <= 448 as an e4m3 code, rounded up or down by 16 random bits: the bits that a code keeps are the float's own above bit 20; below the smallest normal
-// code (2^-6) all steps are 2^-9, which adding 2^-6 makes them in the float too.
+// code (2^-6) all steps are 2^-9, which adding 2^-6 makes them in the float too.  (Where a warp has only normal codes it makes them four bits higher up, with
+// the exponents' difference, 120 << 27 = -0x40000000, in the top byte of the random bits: three instructions a code, and the bytes are picked from the tops.)
 __device__ __forceinline__ unsigned to_code(float y, unsigned bits16) {
     const bool small = y < 0.015625f;
     const float z = small ? y + 0.015625f : y;
     return ((__float_as_uint(z) + (bits16 << 4)) >> 20) - (small ? 121u << 3 : 120u << 3);
 }
-__device__ __forceinline__ float from_code(unsigned char c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+__device__ __forceinline__ float reciprocal_fast(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float reciprocal_root_fast(float v) { float r; asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float min3(float a, float b, float c) { float r; asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ Two negative2(float v) { return two(-v, -v); }
+
+// Quotients and roots the way of Markstein (1990): an approximation, and its remainder, which a fused multiply-add has exactly, to correct it.
+// a / b for |a| <= 448 b; `by` = 1 / b, b in 2^-100 .. 2^100.
+__device__ __forceinline__ Two divide2(Two a, float b, float by) {
+    const Two by2 = two(by, by), q = mul2(a, by2);
+    return fma2(fma2(q, negative2(b), a), by2, q);
+}
+__device__ __forceinline__ float reciprocal(float b) { const float r = reciprocal_fast(b); return fmaf(r, fmaf(-b, r, 1.0f), r); }
+// Zero stays zero; below 2^-100 the root is only about right.
+__device__ __forceinline__ Two root2(Two v) {
+    float a, b;
+    apart(add2(v, two(1e-37f, 1e-37f)), a, b);
+    const Two r = two(reciprocal_root_fast(a), reciprocal_root_fast(b)), q = mul2(v, r), rest = fma2(mul2(q, two(-1.0f, -1.0f)), q, v);
+    return fma2(rest, mul2(r, two(0.5f, 0.5f)), q);
 }
 
+// A block of threads takes a piece, a warp a block of it, a lane eight values.  Every product and sum of the moments is rounded by itself, and the roots and
+// quotients that become codes are correctly rounded (but for one in thousands, off by the last bit): codes do not depend on what a compiler fuses.
 template <int BITS>
-__global__ void __launch_bounds__(THREADS) k_adamw(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, Settings s, float lr, float grad_scale) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, const __grid_constant__ Settings s, float lr, float grad_scale) {
+    extern __shared__ __align__(128) unsigned char shared_bytes[];
+    Ring<BITS>& ring = *reinterpret_cast<Ring<BITS>*>(shared_bytes);
+    init_ring(ring);
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
-    const long long step = ctl->step;
-    const bool go = !s.clipped || ctl->go;
-    const float fix1 = (float)(1.0 / (1.0 - ctl->power1)), fix2 = (float)(1.0 / (1.0 - ctl->power2));
-    const float scale = s.clipped ? grad_scale * ctl->clip : grad_scale;
-    for (unsigned k = blockIdx.x * WARPS + warp; go && k < n; k += gridDim.x * WARPS) {
-        const Piece pc = pieces[k];
-        const Tensor& t = tensors[pc.tensor];
-        const long long from = (long long)pc.block * BLOCK;
-        const int len = (int)min((long long)BLOCK, t.count - from);
-        float m[8], v[8], scale1 = 0.0f, scale2 = 0.0f;
-        if (BITS == 8) { scale1 = t.scale1[pc.block]; scale2 = t.scale2[pc.block]; }
-        float top1 = 0.0f, top2 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = (int)lane + 32 * i;
-            m[i] = v[i] = 0.0f;
-            if (j >= len) continue;
-            const long long at = from + j;
-            const float g = load(t.grad, t.grad_type, at) * scale;
-            float w = t.master ? t.master[at] : load(t.param, t.param_type, at);
-            if (BITS == 32) { m[i] = static_cast<float*>(t.moment1)[at]; v[i] = static_cast<float*>(t.moment2)[at]; }
-            else {
-                m[i] = from_code(static_cast<unsigned char*>(t.moment1)[at]) * scale1;
-                const float root = from_code(static_cast<unsigned char*>(t.moment2)[at]) * scale2;
-                v[i] = root * root;
-            }
-            m[i] = s.beta1 * m[i] + s.rest1 * g;
-            v[i] = s.beta2 * v[i] + s.rest2 * g * g;
-            w -= lr * t.lr_scale * (t.decay * w + m[i] * fix1 / (sqrtf(v[i] * fix2) + s.eps));
-            if (t.master) t.master[at] = w;
-            store(t.param, t.param_type, at, w);
-            if (BITS == 32) { static_cast<float*>(t.moment1)[at] = m[i]; static_cast<float*>(t.moment2)[at] = v[i]; }
-            else { v[i] = sqrtf(v[i]); top1 = fmaxf(top1, fabsf(m[i])); top2 = fmaxf(top2, v[i]); }
+    const bool copies = warp == WARPS;
+    if (copies) copy_pieces(ring, tensors, pieces, n, ctl);                  // (what it copies is not what the norm's kernel writes)
+    asm volatile("griddepcontrol.wait;" ::: "memory");                       // for the norm, when there is one
+    const long long step = __ldcg(&ctl->step);
+    const float fix1 = __ldcg(&ctl->fix1), root_fix2 = __ldcg(&ctl->root_fix2);
+    const bool go = !s.clipped || __ldcg(&ctl->go);
+    const float scale = s.clipped ? grad_scale * __ldcg(&ctl->clip) : grad_scale;
+    unsigned place = 0u, parity = 0u;
+    for (unsigned long long k = blockIdx.x; k < n && !copies; k += gridDim.x) {
+        Stage<BITS>& st = ring.stage[place];
+        unsigned long long* const empty = &ring.empty[place];
+        if (!mbar_wait(&ring.full[place], parity, 0u)) { if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT); break; }
+        if (++place == Ring<BITS>::STAGES) { place = 0u; parity ^= 1u; }
+        const Piece pc = st.piece;
+        if (warp >= pc.blocks || !go) {
+            __syncwarp();
+            if (lane == 0u) mbar_arrive(empty);
+            continue;
         }
+        const Tensor t = st.tensor;
+        const unsigned block = pc.block + warp;
+        const long long at = (long long)block * BLOCK + lane * 8u;
+        const int len = (int)min(8ll, t.count - at);                         // of this lane's eight
+        const bool wide = t.wide && len == 8;
+        const int grad_type = t.grad_type, param_type = t.param_type;
+        float* const master = t.master;
+        void* const param = t.param;
+        void* const moment1 = t.moment1;
+        void* const moment2 = t.moment2;
+        float* const at_scale1 = t.scale1 + block;
+        float* const at_scale2 = t.scale2 + block;
+        const float rate = lr * t.lr_scale, decay = t.decay;
+        const int weight_type = master ? CUDARL_F32 : param_type;
+        Raw gr, wr, mr, vr;
+        uint2 c1 = make_uint2(0u, 0u), c2 = c1;
+        float old1 = 0.0f, old2 = 0.0f;
+        if (warp < copied_blocks<BITS>(t, pc)) {
+            unstage8(gr, st.g, grad_type, warp, lane);
+            unstage8(wr, st.w, weight_type, warp, lane);
+            if (BITS == 32) { unstage8(mr, st.m, CUDARL_F32, warp, lane); unstage8(vr, st.v, CUDARL_F32, warp, lane); }
+            else { c1 = reinterpret_cast<const uint2*>(st.m)[warp * 32u + lane]; c2 = reinterpret_cast<const uint2*>(st.v)[warp * 32u + lane]; }
+        } else {
+            load8(gr, t.grad, grad_type, at, false, len);
+            load8(wr, master ? master : param, weight_type, at, false, len);
+            if (BITS == 32) { load8(mr, moment1, CUDARL_F32, at, false, len); load8(vr, moment2, CUDARL_F32, at, false, len); }
+            else { c1 = load_codes(moment1, at, false, len); c2 = load_codes(moment2, at, false, len); }
+        }
+        if (BITS == 8) { old1 = st.scale1[warp]; old2 = st.scale2[warp]; }
+        __syncwarp();
+        if (lane == 0u) mbar_arrive(empty);                                  // the stage can be filled again
+        float g[8], w[8], m[8], v[8];
+        floats8(gr, grad_type, g);
+        floats8(wr, weight_type, w);
+        if (BITS == 32) { floats8(mr, CUDARL_F32, m); floats8(vr, CUDARL_F32, v); }
         if (BITS == 8) {
-            scale1 = warp_max(top1) / 448.0f; scale2 = warp_max(top2) / 448.0f;
-            if (lane == 0) { t.scale1[pc.block] = scale1; t.scale2[pc.block] = scale2; }
+            from_codes(c1.x, m); from_codes(c1.y, m + 4); from_codes(c2.x, v); from_codes(c2.y, v + 4);
+            const Two s1 = two(old1, old1), s2 = two(old2, old2);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int j = (int)lane + 32 * i;
-                if (j >= len) continue;
-                const unsigned long long quad = (unsigned long long)k * (BLOCK / 4) + (unsigned)j / 4u;
-                const U4 r = philox4x32_10((unsigned)quad, (unsigned)(quad >> 32), (unsigned)(step + 1), (unsigned)((unsigned long long)(step + 1) >> 32), s.k0, s.k1);
-                const unsigned word = j % 4 == 0 ? r.x : j % 4 == 1 ? r.y : j % 4 == 2 ? r.z : r.w;
-                const unsigned c1 = to_code(fminf(fabsf(m[i]) / (scale1 > 0.0f ? scale1 : 1.0f), 448.0f), word & 0xFFFFu);
-                unsigned c2 = to_code(fminf(v[i] / (scale2 > 0.0f ? scale2 : 1.0f), 448.0f), word >> 16);
-                if (c2 == 0u && v[i] > 0.0f) c2 = 1u;
-                static_cast<unsigned char*>(t.moment1)[from + j] = (unsigned char)(c1 | (m[i] < 0.0f ? 128u : 0u));
-                static_cast<unsigned char*>(t.moment2)[from + j] = (unsigned char)c2;
+            for (int i = 0; i < 8; i += 2) {
+                apart(mul2(two(m[i], m[i + 1]), s1), m[i], m[i + 1]);
+                const Two r = mul2(two(v[i], v[i + 1]), s2);
+                apart(mul2(r, r), v[i], v[i + 1]);
             }
+        }
+        float root[8];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const Two gi = mul2(two(g[i], g[i + 1]), two(scale, scale));
+            const Two mi = add2(mul2(two(s.beta1, s.beta1), two(m[i], m[i + 1])), mul2(two(s.rest1, s.rest1), gi));
+            const Two vi = add2(mul2(two(s.beta2, s.beta2), two(v[i], v[i + 1])), mul2(mul2(two(s.rest2, s.rest2), gi), gi)), ri = root2(vi);
+            float a, b;
+            apart(fma2(ri, two(root_fix2, root_fix2), two(s.eps, s.eps)), a, b);
+            const Two wi = two(w[i], w[i + 1]), way = mul2(mul2(mi, two(fix1, fix1)), two(reciprocal_fast(a), reciprocal_fast(b)));
+            apart(fma2(negative2(rate), fma2(two(decay, decay), wi, way), wi), w[i], w[i + 1]);
+            apart(mi, m[i], m[i + 1]); apart(vi, v[i], v[i + 1]); apart(ri, root[i], root[i + 1]);
+        }
+        if (master) store8(master, CUDARL_F32, at, wide, len, w);
+        store8(param, param_type, at, wide, len, w);
+        if (BITS == 32) {
+            store8(moment1, CUDARL_F32, at, wide, len, m);
+            store8(moment2, CUDARL_F32, at, wide, len, v);
+        } else {
+            // the largest magnitudes, in the order of their bits (values behind the tensor's end are zeros; NaN is the largest)
+            float top1 = 0.0f, top2 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) { top1 = max_nan(top1, fabsf(m[i]), fabsf(m[i + 1])); top2 = max_nan(top2, root[i], root[i + 1]); }
+            const float scale1 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top1))) * (1.0f / 448.0f), scale2 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top2))) * (1.0f / 448.0f);
+            if (lane == 0) { *at_scale1 = scale1; *at_scale2 = scale2; }
+            float y1[8], y2[8], least = 448.0f;
+            const bool usual = scale1 > 7.9e-31f && scale1 < 1.2e30f && scale2 > 7.9e-31f && scale2 < 1.2e30f;
+            if (usual) {
+                const float by1 = reciprocal(scale1), by2 = reciprocal(scale2);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    apart(divide2(two(m[i], m[i + 1]), scale1, by1), y1[i], y1[i + 1]);
+                    apart(divide2(two(root[i], root[i + 1]), scale2, by2), y2[i], y2[i + 1]);
+                    least = min3(min3(least, fabsf(y1[i]), fabsf(y1[i + 1])), y2[i], y2[i + 1]);
+                }
+            } else {
+                const float by1 = scale1 > 0.0f ? scale1 : 1.0f, by2 = scale2 > 0.0f ? scale2 : 1.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { y1[i] = m[i] / by1; y2[i] = root[i] / by2; }
+            }
+            const bool all_normal = __all_sync(~0u, usual && least >= 0.015625f);
+            unsigned d1[2], d2[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const unsigned long long quad = (unsigned long long)(pc.number + warp) * (BLOCK / 4) + lane * 2u + q;
+                const U4 r = philox4x32_10((unsigned)quad, (unsigned)(quad >> 32), (unsigned)(step + 1), (unsigned)((unsigned long long)(step + 1) >> 32), s.keys);
+                const unsigned word[4] = {r.x, r.y, r.z, r.w};
+                unsigned a[4], b[4];                                         // a code in the top byte of each
+                if (all_normal) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * q + i;
+                        a[i] = (__float_as_uint(y1[e]) << 4) + __byte_perm(word[i], 0x40000000u, 0x7104u) | __float_as_uint(m[e]) & 0x80000000u;
+                        b[i] = (__float_as_uint(y2[e]) << 4) + __byte_perm(word[i], 0x40000000u, 0x7324u);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * q + i;
+                        a[i] = to_code(fminf(fabsf(y1[e]), 448.0f), word[i] & 0xFFFFu) << 24 | __float_as_uint(m[e]) & 0x80000000u;
+                        b[i] = max(to_code(fminf(y2[e], 448.0f), word[i] >> 16), root[e] > 0.0f ? 1u : 0u) << 24;
+                    }
+                }
+                d1[q] = __byte_perm(__byte_perm(a[0], a[1], 0x0073u), __byte_perm(a[2], a[3], 0x0073u), 0x5410u);
+                d2[q] = __byte_perm(__byte_perm(b[0], b[1], 0x0073u), __byte_perm(b[2], b[3], 0x0073u), 0x5410u);
+            }
+            store_codes(moment1, at, wide, len, make_uint2(d1[0], d1[1]));
+            store_codes(moment2, at, wide, len, make_uint2(d2[0], d2[1]));
         }
     }
     if (last_block(&ctl->done)) {
-        if (go) { ctl->step = step + 1; ctl->power1 *= s.power1; ctl->power2 *= s.power2; }
-        else ctl->skipped += 1;
+        if (go) {
+            const double p1 = ctl->power1 * s.power1, p2 = ctl->power2 * s.power2;
+            ctl->step = step + 1; ctl->power1 = p1; ctl->power2 = p2;
+            ctl->fix1 = (float)(1.0 / (1.0 - p1)); ctl->root_fix2 = (float)sqrt(1.0 / (1.0 - p2));
+        } else ctl->skipped += 1;
     }
 }
 
@@ -188,6 +496,8 @@ struct cudarl_adamw {
 };
 
 namespace {
+
+size_t ring_bytes(int bits) { return bits == 8 ? sizeof(Ring<8>) : bits == 32 ? sizeof(Ring<32>) : sizeof(Ring<0>); }
 
 int check_tensor(const cudarl_adamw_tensor& t, int bits, CallerArrays& arrays) {
     if (t.count < 0 || t.count > (1ll << 40)) return fail_global(-1, "count of a tensor out of range");
@@ -223,26 +533,38 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
     CallerArrays arrays;
     arrays.expect(o->cfg.device);
     std::vector<Piece> pieces;
+    int64_t number = 0;
     for (int32_t i = 0; i < count; ++i) {
         const cudarl_adamw_tensor& t = tensors[i];
         const int rc = check_tensor(t, o->cfg.state_bits, arrays);
         if (rc) return rc;
-        o->tensors.push_back(Tensor{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.param_type, t.grad_type, t.lr_scale, t.weight_decay});
+        Tensor d{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.lr_scale, t.weight_decay, (unsigned char)t.param_type, (unsigned char)t.grad_type, 0, 0, 0};
+        auto eight = [](const void* p, size_t value) { return reinterpret_cast<uintptr_t>(p) % (8 * value) == 0; };
+        auto sixteen = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+        const size_t moment = o->cfg.state_bits == 8 ? 1 : 4;
+        d.wide = eight(t.param, type_bytes(t.param_type)) && eight(t.master, 4) && sixteen(t.moment1) && sixteen(t.moment2) && eight(t.moment1, moment) && eight(t.moment2, moment);
+        d.wide_grad = sixteen(t.grad);
+        o->tensors.push_back(d);
         const int64_t blocks = (t.count + BLOCK - 1) / BLOCK;
-        if ((int64_t)pieces.size() + blocks > (1ll << 31)) return fail_global(-1, "more than 2^39 values in one handle");
-        for (int64_t b = 0; b < blocks; ++b) pieces.push_back(Piece{(unsigned)i, (unsigned)b});
+        if (number + blocks > (1ll << 31)) return fail_global(-1, "more than 2^39 values in one handle");
+        for (int64_t b = 0; b < blocks; b += WARPS) pieces.push_back(Piece{(unsigned)i, (unsigned)b, (unsigned)std::min<int64_t>(WARPS, blocks - b), (unsigned)(number + b)});
+        number += blocks;
     }
     note_gradients(o);
     o->pieces = (unsigned)pieces.size();
+    const int bits = o->cfg.state_bits;
+    if ((e = bits == 32 ? cudaFuncSetAttribute(k_adamw<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_bytes(32))
+                        : cudaFuncSetAttribute(k_adamw<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_bytes(8))) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, o->cfg.device)) != cudaSuccess) return fail_cuda("cudaDeviceGetAttribute", e);
-    const unsigned most = (unsigned)sms * 8u, blocks = (o->pieces + WARPS - 1) / WARPS;
+    const unsigned most = (unsigned)(sms * RESIDENT), blocks = o->pieces;
     o->grid = blocks < 1u ? 1u : blocks < most ? blocks : most;
     Control c;
     std::memset(&c, 0, sizeof c);
     c.step = o->cfg.step;
     c.power1 = std::pow(o->cfg.beta1, (double)(c.step + 1));
     c.power2 = std::pow(o->cfg.beta2, (double)(c.step + 1));
+    c.fix1 = (float)(1.0 / (1.0 - c.power1)); c.root_fix2 = (float)std::sqrt(1.0 / (1.0 - c.power2));
     c.clip = 1.0f;
     if ((e = cudaMalloc(&o->dtensors, sizeof(Tensor) * (o->tensors.size() + 1))) != cudaSuccess || (e = cudaMalloc(&o->dpieces, sizeof(Piece) * (pieces.size() + 1))) != cudaSuccess ||
         (e = cudaMalloc(&o->dctl, sizeof(Control))) != cudaSuccess || (e = cudaMalloc(&o->dpart, sizeof(double) * o->grid)) != cudaSuccess) return fail_cuda("cudaMalloc", e);
@@ -292,12 +614,27 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
     if (e != cudaSuccess) return fail_cuda("cudaSetDevice", e);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudarl_adamw_config& c = o->cfg;
-    const Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, (unsigned)c.seed, (unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER,
-                     c.max_grad_norm > 0.0f, c.beta1, c.beta2};
-    if (s.clipped) k_grad_norm<<<o->grid, THREADS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, grad_scale, c.max_grad_norm);
-    if (c.state_bits == 32) k_adamw<32><<<o->grid, THREADS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, s, lr, grad_scale);
-    else k_adamw<8><<<o->grid, THREADS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, s, lr, grad_scale);
-    e = cudaGetLastError();
+    Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, {}, c.max_grad_norm > 0.0f, c.beta1, c.beta2};
+    for (unsigned r = 0; r < 10; ++r) {
+        s.keys[2 * r] = (unsigned)c.seed + r * 0x9E3779B9u;
+        s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;
+    }
+    if (s.clipped) {
+        k_grad_norm<<<o->grid, THREADS, ring_bytes(0), st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, grad_scale, c.max_grad_norm);
+        if ((e = cudaGetLastError()) != cudaSuccess) return fail_cuda("cudarl_adamw_step", e);
+    }
+    cudaLaunchConfig_t launch = {};
+    launch.gridDim = dim3(o->grid); launch.blockDim = dim3(THREADS); launch.stream = st;
+    launch.dynamicSmemBytes = ring_bytes(c.state_bits);
+    // after the norm's kernel: started while that one still runs, its first loads done, it waits for the norm on the device.  Without a norm it must not begin
+    // before the gradients' own kernel has ended
+    cudaLaunchAttribute early[1];
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; early[0].val.programmaticStreamSerializationAllowed = 1;
+    if (s.clipped) { launch.attrs = early; launch.numAttrs = 1; }
+    const Tensor* tensors = o->dtensors;
+    const Piece* pieces = o->dpieces;
+    e = c.state_bits == 32 ? cudaLaunchKernelEx(&launch, k_adamw<32>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale)
+                           : cudaLaunchKernelEx(&launch, k_adamw<8>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale);
     return e == cudaSuccess ? 0 : fail_cuda("cudarl_adamw_step", e);
 }
 
@@ -318,7 +655,11 @@ extern "C" int cudarl_adamw_set_gradients(cudarl_adamw* o, const void* const* gr
         const int rc = arrays.check("grad", grads[i], type_bytes(o->tensors[i].grad_type));
         if (rc) return rc;
     }
-    for (size_t i = 0; i < o->tensors.size(); ++i) o->tensors[i].grad = grads[i];
+    for (size_t i = 0; i < o->tensors.size(); ++i) {
+        Tensor& t = o->tensors[i];
+        t.grad = grads[i];
+        t.wide_grad = reinterpret_cast<uintptr_t>(t.grad) % 16 == 0;
+    }
     note_gradients(o);
     // the copy is from pageable memory: it has been taken from there when the call returns
     if (!o->tensors.empty() && (e = cudaMemcpyAsync(o->dtensors, o->tensors.data(), sizeof(Tensor) * o->tensors.size(), cudaMemcpyHostToDevice, st)) != cudaSuccess) return fail_cuda("cudaMemcpyAsync", e);
@@ -333,5 +674,6 @@ extern "C" int cudarl_adamw_get_stats(cudarl_adamw* o, cudarl_adamw_stats* out) 
     Control c;
     if ((e = cudaDeviceSynchronize()) != cudaSuccess || (e = cudaMemcpy(&c, o->dctl, sizeof c, cudaMemcpyDeviceToHost)) != cudaSuccess) return fail_cuda("cudarl_adamw_get_stats", e);
     out->step = c.step; out->skipped = c.skipped; out->grad_norm = c.norm;
+    if (c.error) return fail_global(CUDARL_ERR_DEVICE + (int)c.error, "a wait of the optimizer's kernel ran out: its tensors are not to be used");
     return 0;
 }

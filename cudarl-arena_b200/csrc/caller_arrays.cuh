@@ -1,4 +1,4 @@
-// caller_arrays.cuh -- what the entry points on the caller's own device arrays share: where an array is, and loads and stores of its type.
+// caller_arrays.cuh -- what the entry points on the caller's own device arrays share: where an array is, its types, and the arithmetic on two floats at once.
 #pragma once
 #include "internal.h"
 #include <cuda_bf16.h>
@@ -88,5 +88,13 @@ template <> struct Of<CUDARL_F16> {
     static __device__ __forceinline__ float get(T v) { return __half2float(v); }
     static __device__ __forceinline__ T put(float v) { return __float2half_rn(v); }
 };
+
+// Two floats for the instructions that take two: half as many to issue, each of the two rounded as by itself.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void apart(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ Two add2(Two a, Two b) { Two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ Two mul2(Two a, Two b) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 }  // namespace cudarl
