@@ -56,35 +56,41 @@ __device__ __forceinline__ void load8(Raw& r, const void* p, int type, long long
     if (type == CUDARL_F32) {
         const unsigned* at = static_cast<const unsigned*>(p) + i;
         if (wide) asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]), "=r"(r.v[4]), "=r"(r.v[5]), "=r"(r.v[6]), "=r"(r.v[7]) : "l"(at));
-        else
+        else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) r.v[k] = k < len ? at[k] : 0u;
+        }
     } else {
         const unsigned short* at = static_cast<const unsigned short*>(p) + i;
         if (wide) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "l"(at));
-        else
+        else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) r.v[k] = (2 * k < len ? at[2 * k] : 0u) | (2 * k + 1 < len ? (unsigned)at[2 * k + 1] << 16 : 0u);
+        }
     }
 }
 __device__ __forceinline__ void floats8(const Raw& r, int type, float (&x)[8]) {
-    if (type == CUDARL_F32)
+    if (type == CUDARL_F32) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(r.v[k]);
-    else if (type == CUDARL_BF16)
+    }
+    else if (type == CUDARL_BF16) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) { x[2 * k] = __uint_as_float(r.v[k] << 16); x[2 * k + 1] = __uint_as_float(r.v[k] & 0xFFFF0000u); }
-    else
+    }
+    else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.v[k])); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
+    }
 }
 __device__ __forceinline__ void store8(void* p, int type, long long i, bool wide, int len, const float (&x)[8]) {
     if (type == CUDARL_F32) {
         float* at = static_cast<float*>(p) + i;
         if (wide) asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" :: "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]), "l"(at) : "memory");
-        else
+        else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) if (k < len) at[k] = x[k];
+        }
         return;
     }
     unsigned v[4];
@@ -153,7 +159,6 @@ template <int BITS> struct Ring {
 static_assert(sizeof(Tensor) % 16 == 0 && sizeof(Piece) % 16 == 0 && sizeof(Ring<8>) % 16 == 0 && sizeof(Stage<8>) % 16 == 0 && sizeof(Stage<32>) % 16 == 0 && sizeof(Stage<0>) % 16 == 0,
               "bulk copies take multiples of 16 bytes");
 __device__ __forceinline__ void copy4(void* to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(to)), "l"(from) : "memory"); }
-__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory"); }
 
 // Of a piece: how many of its blocks come by copies.
 template <int BITS> __device__ __forceinline__ unsigned copied_blocks(const Tensor& t, const Piece& pc) {

@@ -10,6 +10,7 @@
 // test.  Rows with |m c| of 2^23 and more, where the error would be whole powers of two, are gone through a second time with exact differences.
 #include "caller_arrays.cuh"
 #include <cooperative_groups.h>
+#include <cstdlib>
 
 namespace {
 using namespace cudarl;
@@ -35,6 +36,7 @@ struct Outputs {
 // ------------------------------------------------------------------------------------------------------------------ arithmetic
 __device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 // Larger for the larger logit, of equal ones for the lower action; 0 for none.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned action) {
     const unsigned b = __float_as_uint(x + 0.0f);                            // -0 counts as 0
@@ -63,12 +65,6 @@ __device__ __forceinline__ void take_one(Part& p, float x, float c) {
     p.s += e;
     p.t = fmaf(y, e, p.t);
 }
-__device__ __forceinline__ void join(Part& a, Part b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    rebase(a, m, c); rebase(b, m, c);
-    a.s += b.s; a.t += b.t;
-}
-
 // What is known of a whole row.
 struct Known {
     float m, log2_s, h;
@@ -210,85 +206,91 @@ __device__ __forceinline__ void take32(unsigned long long& list, unsigned long l
     if (__any_sync(ALL, key > least)) list = merged32(list, sorted32(key, lane), lane);
 }
 
+__device__ __forceinline__ void write_top(const Outputs& o, const Rows& p, const Known& known, long long r, int place, unsigned long long key) {
+    o.top_actions[r * o.top + place] = key ? key_action(key) : -1;
+    o.top_logprobs[r * o.top + place] = known.bad ? known.log2_s : key ? known.logprob(key_value(key), p) : NONE;
+}
+
 // ------------------------------------------------------------------------------------------------------------------ short rows
-// G lanes a row, E values a lane in registers: up to G E actions.  The sums of a row need log2(G) exchanges; every load of a lane is one 16- or 32-byte
-// piece where rows are aligned to it.
-template <int TYPE, int E>
-__device__ __forceinline__ void load_short(const Rows& p, long long r, int j0, bool wide, float (&x)[E]) {
+// G lanes a row, E values a lane in registers: up to G E actions.  WIDE: a lane has neighbouring values and moves them at once, which takes rows that are aligned
+// to that; else neighbouring lanes have neighbouring values, so that what a warp reads or writes at a time lies together.
+template <int G, int E, bool WIDE> __device__ __forceinline__ int short_action(int lane, int i) { return WIDE ? lane * E + i : lane + G * i; }
+
+template <int TYPE, int G, int E, bool WIDE>
+__device__ __forceinline__ void load_short(const Rows& p, long long r, int lane, float (&x)[E]) {
     using O = Of<TYPE>;
-    const auto* at = static_cast<const typename O::T*>(p.logits) + r * p.stride + j0;
-    if (wide && j0 + E <= p.actions) {
-        constexpr int BYTES = E * (int)sizeof(typename O::T);
-        if constexpr (BYTES == 8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(at);
+    const auto* at = static_cast<const typename O::T*>(p.logits) + r * p.stride;
+    constexpr int BYTES = E * (int)sizeof(typename O::T);
+    if (WIDE && lane * E + E <= p.actions) {
+        if constexpr (BYTES == 8 && TYPE != CUDARL_F32) {
+            const uint2 v = *reinterpret_cast<const uint2*>(at + lane * E);
             Chunk<TYPE>::pair(v.x, x[0], x[1]); Chunk<TYPE>::pair(v.y, x[2], x[3]);
-        } else {
+        } else if constexpr (BYTES >= 16) {
 #pragma unroll
             for (int k = 0; k < BYTES / 16; ++k) {
                 float part[Chunk<TYPE>::N];
-                Chunk<TYPE>::values(reinterpret_cast<const uint4*>(at)[k], part);
+                Chunk<TYPE>::values(reinterpret_cast<const uint4*>(at + lane * E)[k], part);
 #pragma unroll
                 for (int i = 0; i < Chunk<TYPE>::N; ++i) x[k * Chunk<TYPE>::N + i] = part[i];
             }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = j0 + i < p.actions ? O::get(at[i]) : NONE;
+        for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); x[i] = j < p.actions ? O::get(at[j]) : NONE; }
+    }
+    if (p.legal) {
+        const unsigned char* legal = p.legal + r * p.legal_stride;
+#pragma unroll
+        for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); x[i] = j < p.actions && __ldg(legal + j) ? x[i] : NONE; }
     }
 }
-template <int E>
-__device__ __forceinline__ void mask_short(const Rows& p, long long r, int j0, unsigned& bits) {
-    const unsigned char* legal = p.legal + r * p.legal_stride + j0;
-    bits = 0u;
+
+// y and 2^y of the lane's values, and the row's part in all its lanes.
+template <int G, int E>
+__device__ __forceinline__ Part sum_short(const float (&x)[E], float scale, float (&y)[E], float (&e)[E]) {
+    float m = x[0];
 #pragma unroll
-    for (int i = 0; i < E; ++i) bits |= j0 + i < p.actions && __ldg(legal + i) ? 1u << i : 0u;
+    for (int i = 1; i < E; ++i) m = fmaxf(m, x[i]);
+#pragma unroll
+    for (int by = 1; by < G; by *= 2) m = fmaxf(m, __shfl_xor_sync(ALL, m, by));
+    const float c = scale * LOG2E, mc = m * c, from = m == NONE ? 0.0f : m;
+    const bool exact = !is_usual(m, c);
+    Part part{m, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        y[i] = fmaf(max_nan(x[i], FLOOR), c, -mc);
+        if (exact) y[i] = max_nan((x[i] - from) * scale * LOG2E, FLOOR);
+        e[i] = exp2_fast(y[i]);
+        part.s += e[i];
+        part.t = fmaf(y[i], e[i], part.t);
+    }
+#pragma unroll
+    for (int by = 1; by < G; by *= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
+    return part;
 }
 
-template <int TYPE, int G, int E, bool TOP>
-__global__ void __launch_bounds__(256) k_short(Rows p, Outputs o, bool wide) {
-    const int lane = (int)threadIdx.x % G, j0 = lane * E;
+template <int TYPE, int G, int E, bool WIDE, bool TOP>
+__global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
+    const int lane = (int)threadIdx.x % G;
     const long long step = (long long)gridDim.x * (256 / G);
     // (the loop is the same for all lanes of a warp: rows behind the last are computed from the last and not written)
     for (long long first = (long long)blockIdx.x * (256 / G); first < p.rows; first += step) {
         const long long mine = first + (int)threadIdx.x / G, r = mine < p.rows ? mine : p.rows - 1;
         const bool write = mine < p.rows;
-        float x[E];
-        load_short<TYPE, E>(p, r, j0, wide, x);
-        if (p.legal) {
-            unsigned bits;
-            mask_short<E>(p, r, j0, bits);
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = bits >> i & 1u ? x[i] : NONE;
-        }
+        float x[E], y[E], e[E];
+        load_short<TYPE, G, E, WIDE>(p, r, lane, x);
         const int a = p.taken ? __ldg(p.taken + r) : -1;
-        float m = x[0];
-#pragma unroll
-        for (int i = 1; i < E; ++i) m = fmaxf(m, x[i]);
-#pragma unroll
-        for (int by = 1; by < G; by *= 2) m = fmaxf(m, __shfl_xor_sync(ALL, m, by));
-        const float c = p.scale * LOG2E, mc = m * c, from = m == NONE ? 0.0f : m;
-        const bool exact = !is_usual(m, c);
-        Part part{m, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            float y = fmaf(max_nan(x[i], FLOOR), c, -mc);
-            if (exact) y = (x[i] - from) * p.scale * LOG2E;
-            const float e = exp2_fast(y);
-            part.s += e;
-            part.t += e > 0.0f ? y * e : 0.0f;
-        }
-#pragma unroll
-        for (int by = 1; by < G; by *= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
-        const Known known(part);
+        const Known known(sum_short<G, E>(x, p.scale, y, e));
         if (write) {
-            if (lane == 0) known.write(o, r);
+            if (lane == 0 && o.entropy) o.entropy[r] = known.h;
             if (o.logprob) {
                 if ((unsigned)a >= (unsigned)p.actions) { if (lane == 0) o.logprob[r] = known.bad ? known.log2_s : 0.0f; }
-                else if ((unsigned)(a - j0) < (unsigned)E) {                 // the lane that holds it
+                else {
                     float xa = x[0];
+                    bool has = a == short_action<G, E, WIDE>(lane, 0);
 #pragma unroll
-                    for (int i = 1; i < E; ++i) xa = a - j0 == i ? x[i] : xa;
-                    o.logprob[r] = known.logprob(xa, p);
+                    for (int i = 1; i < E; ++i) { const bool is = a == short_action<G, E, WIDE>(lane, i); xa = is ? x[i] : xa; has = has || is; }
+                    if (has) o.logprob[r] = known.logprob(xa, p);            // the lane that holds it
                 }
             }
         }
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o, bool wide) {
             // every lane's own values in falling order, then the largest head of the G lists, `top` times
             unsigned long long key[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) key[i] = x[i] > NONE && !known.bad ? order_key(x[i], (unsigned)(j0 + i)) : 0ull;
+            for (int i = 0; i < E; ++i) key[i] = x[i] > NONE && !known.bad ? order_key(x[i], (unsigned)short_action<G, E, WIDE>(lane, i)) : 0ull;
 #pragma unroll
             for (int size = 2; size <= E; size *= 2)
 #pragma unroll
@@ -314,10 +316,7 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o, bool wide) {
 #pragma unroll
                 for (int by = 1; by < G; by *= 2) { const unsigned long long other = __shfl_xor_sync(ALL, best, by); best = best > other ? best : other; }
                 if (best == 0ull ? lane == 0 : key[0] == best) {
-                    if (write) {
-                        o.top_actions[r * o.top + k] = best ? key_action(best) : -1;
-                        o.top_logprobs[r * o.top + k] = known.bad ? known.log2_s : best ? known.logprob(key_value(best), p) : NONE;
-                    }
+                    if (write) write_top(o, p, known, r, k, best);
 #pragma unroll
                     for (int i = 0; i + 1 < E; ++i) key[i] = key[i + 1];
                     key[E - 1] = 0ull;
@@ -327,258 +326,416 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o, bool wide) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------ parts of warps
+__device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float warp_min(float v) { float r; asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+// The 32 lanes' parts as one, in every lane.
+__device__ __forceinline__ void join_lanes(Part& p, float c, int lanes = 32) {
+    rebase(p, warp_max(p.m), c);
+    for (int by = lanes / 2; by; by /= 2) { p.s += __shfl_xor_sync(ALL, p.s, by); p.t += __shfl_xor_sync(ALL, p.t, by); }
+}
+// The `rank`-th largest of the lanes' values (1 .. 32).
+__device__ __forceinline__ float warp_ranked(float v, int rank, unsigned lane) {
+    float high = NONE;
+    for (int k = 0; k < rank; ++k) {
+        high = warp_max(v);
+        if (lane == (unsigned)__ffs((int)__ballot_sync(ALL, v == high)) - 1u) v = NONE;
+    }
+    return high;
+}
+// A whole row by the threads of a team the slow way, with exact differences: lane- and warp-wise parts of it (see below for where it is needed).
+template <int TYPE> __device__ __forceinline__ float exact_max(const Row<TYPE>& row, int t, int threads) {
+    float m = NONE;
+    for (int j = t; j < row.actions; j += threads) m = fmaxf(m, row.at(j));
+    return warp_max(m);
+}
+template <int TYPE> __device__ __forceinline__ Part exact_sums(const Row<TYPE>& row, float m, float scale, int t, int threads) {
+    const float from = m == NONE ? 0.0f : m;
+    Part p{m, 0.0f, 0.0f};
+    for (int j = t; j < row.actions; j += threads) {
+        const float y = (row.at(j) - from) * scale * LOG2E, e = exp2_fast(y);
+        p.s += e;
+        p.t += e > 0.0f ? y * e : 0.0f;
+    }
+#pragma unroll
+    for (int by = 16; by; by /= 2) { p.s += __shfl_xor_sync(ALL, p.s, by); p.t += __shfl_xor_sync(ALL, p.t, by); }
+    return p;
+}
+// The best of a row by one warp that goes through all its values, 32 at a time.
+template <int TYPE> __device__ __forceinline__ unsigned long long best_of_all(const Row<TYPE>& row, int first, int step, unsigned lane, int top) {
+    unsigned long long best = 0ull;
+    for (int j0 = first; j0 < row.actions; j0 += step) {
+        const int j = j0 + (int)lane;
+        const float x = j < row.actions ? row.at(j) : NONE;
+        take32(best, x > NONE ? order_key(x, (unsigned)j) : 0ull, lane, top);
+    }
+    return best;
+}
+// How many of n keys are larger than this one: its place in the order.
+__device__ __forceinline__ int place_of(unsigned long long key, const unsigned long long* keys, int n) {
+    int place = 0;
+    for (int l = 0; l < n; ++l) place += keys[l] > key ? 1 : 0;
+    return place;
+}
+
+template <int TYPE> __device__ __forceinline__ void largest(const float (&x)[Chunk<TYPE>::N], float& m) {
+#pragma unroll
+    for (int i = 0; i < Chunk<TYPE>::N; i += 2) m = max3(m, x[i], x[i + 1]);
+}
+template <int TYPE> __device__ __forceinline__ void add_chunk(const float (&x)[Chunk<TYPE>::N], Two c2, Two mc2, Two& s2, Two& t2) {
+#pragma unroll
+    for (int i = 0; i < Chunk<TYPE>::N; i += 2) {
+        const Two y2 = fma2(two(x[i], x[i + 1]), c2, mc2);
+        float y0, y1;
+        apart(y2, y0, y1);
+        const Two e2 = two(exp2_fast(y0), exp2_fast(y1));
+        s2 = add2(s2, e2);
+        t2 = fma2(y2, e2, t2);
+    }
+}
+__device__ __forceinline__ float sum2(Two v) { float a, b; apart(v, a, b); return a + b; }
+
+// ------------------------------------------------------------------------------------------------------------------ rows of a warp
+// A warp a row, the whole row in registers: CHUNKS pieces of 16 bytes a lane, and an end.  The alternatives: the `top`-th largest of the lanes' maxima is a bound
+// that `top` values reach; the lanes list what reaches it, and each of those counts how many are larger.
+constexpr int WARP_KEYS = 64;
+
+// Blocks on an SM for which the registers suffice.
+constexpr int warp_blocks(int values) { return values <= 8 ? 5 : values <= 16 ? 4 : 3; }
+
+template <int TYPE, int CHUNKS, bool MASKED, bool TOP>
+__global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_warp(Rows p, Outputs o) {
+    using C = Chunk<TYPE>;
+    constexpr int N = C::N;
+    __shared__ unsigned long long keys_all[TOP ? 8 * WARP_KEYS : 1];
+    const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
+    unsigned long long* const keys = keys_all + (TOP ? warp * WARP_KEYS : 0u);
+    const float c = p.scale * LOG2E;
+    const long long step = (long long)gridDim.x * 8;
+    uint4 raw[CHUNKS];
+    unsigned legal[CHUNKS][N / 4];
+    float xe_loaded = NONE;
+    int a_loaded = -1;
+    auto load = [&](const Row<TYPE>& row, long long r) {
+        a_loaded = p.taken ? __ldg(p.taken + r) : -1;
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            const int k = (int)lane + 32 * u;
+            raw[u] = k < row.chunks ? row.chunk(k) : C::fill();
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
+                if (k < row.chunks) mask_words<N>(row.legal, row.head + k * N, row.actions, legal[u]);
+            }
+        }
+        xe_loaded = (int)lane < row.ends ? row.at(row.end((int)lane)) : NONE;
+    };
+    long long r = (long long)blockIdx.x * 8 + warp;
+    if (r < p.rows) load(Row<TYPE>(p, r), r);
+    for (; r < p.rows; r += step) {
+        const Row<TYPE> row(p, r);
+        const int a = a_loaded;
+        const float xe = max_nan(xe_loaded, FLOOR);
+        const bool taken = (unsigned)a < (unsigned)row.actions;
+        const float xa = taken && lane == 0u ? row.at(a) : NONE;
+        float x[CHUNKS][N], m = fmaxf(xe, FLOOR);
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            C::floored(raw[u], x[u]);
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[u][i] = is_legal<N>(legal[u], i) ? x[u][i] : FLOOR;
+            }
+            largest<TYPE>(x[u], m);
+        }
+        if (r + step < p.rows) load(Row<TYPE>(p, r + step), r + step);       // the next row's, on their way while this one is computed
+        const float own = m;
+        m = warp_max(m);
+        Part part{m, 0.0f, 0.0f};
+        if (is_usual(m, c)) {
+            const float mc = base_of(m, c), ye = fmaf(xe, c, -mc), ee = exp2_fast(ye);
+            const Two c2 = two(c, c), mc2 = two(-mc, -mc);
+            Two s2 = two(ee, 0.0f), t2 = two(ye * ee, 0.0f);
+#pragma unroll
+            for (int u = 0; u < CHUNKS; ++u) add_chunk<TYPE>(x[u], c2, mc2, s2, t2);
+            part.s = sum2(s2); part.t = sum2(t2);
+#pragma unroll
+            for (int by = 16; by; by /= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
+        } else {                                                             // beyond the limit
+            m = exact_max(row, (int)lane, 32);
+            part = exact_sums(row, m, p.scale, (int)lane, 32);
+        }
+        const Known known(part);
+        if (lane == 0u) {
+            known.write(o, r);
+            if (o.logprob) o.logprob[r] = known.bad ? known.log2_s : taken ? known.logprob(xa, p) : 0.0f;
+        }
+        if constexpr (TOP) {
+            const float bound = warp_ranked(own, o.top, lane);
+            int n = 0;
+            if (bound > ABOVE_FLOOR && !known.bad) {
+                unsigned mine = 0u;                                          // (values cannot be had from registers by number: they are read again)
+                if (own >= bound) {
+#pragma unroll
+                    for (int u = 0; u < CHUNKS; ++u)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) mine |= x[u][i] >= bound ? 1u << (u * N + i) : 0u;
+                }
+                bool end = xe >= bound;
+                while (true) {
+                    const bool has = mine != 0u || end;
+                    const unsigned who = __ballot_sync(ALL, has);
+                    if (!who) break;
+                    if (has) {
+                        int j;
+                        if (mine) { const int e = __ffs((int)mine) - 1; mine &= mine - 1u; j = row.head + ((int)lane + 32 * (e / N)) * N + e % N; }
+                        else { end = false; j = row.end((int)lane); }
+                        const int place = n + __popc(who & ((1u << lane) - 1u));
+                        if (place < WARP_KEYS) keys[place] = order_key(row.at(j), (unsigned)j);
+                    }
+                    n += __popc(who);
+                }
+                __syncwarp();
+            }
+            if (n >= o.top && n <= WARP_KEYS) {
+                for (int l = (int)lane; l < n; l += 32) {
+                    const unsigned long long key = keys[l];
+                    const int place = place_of(key, keys, n);
+                    if (place < o.top) write_top(o, p, known, r, place, key);
+                }
+            } else {
+                const unsigned long long best = known.bad || known.nothing ? 0ull : best_of_all(row, 0, 32, lane, o.top);
+                if ((int)lane < o.top) write_top(o, p, known, r, (int)lane, best);
+            }
+            __syncwarp();
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------ long rows
-// T threads a row (a warp, or a block), or the blocks of a cluster for few rows.  A thread takes batches of UNROLL chunks; a batch costs one maximum and one
-// rebasing of the thread's sums.  The threads' parts are joined by shuffles, in shared memory, and over the cluster in the other blocks' shared memory.
+// T threads a row, or the blocks of a cluster for few rows.  A thread takes batches of UNROLL chunks; a batch costs one maximum and one rebasing of the thread's
+// sums.  The threads' parts are joined by shuffles, in shared memory, and over the cluster in the other blocks' shared memory.
 //
-// Alternatives: the maximum of every batch (of every GROUP of batches, for very long rows) is kept in shared memory.  With W warps in all, the ceil(top / W)-th
-// largest thread maximum of each warp, and of those the least, is a bound that at least `top` values of the row reach.  Only batches that reach it are read
-// again -- a few dozen of them -- and what reaches the bound there is put in order by one warp.  Where too much does (rows of equal values) or too little (fewer
-// than `top` values above FLOOR), every value of the row is gone through again, each warp with its 32 best in registers.
-constexpr int UNROLL = 4, TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
+// Alternatives: the maximum of every batch (of every GROUP of batches, for very long rows) is kept in shared memory.  32 of the threads' maxima, the largest of each
+// warp, are values of the row, so the `top`-th largest of them is a bound that `top` values reach.  Only batches that reach it are read again -- a few dozen --
+// and of what reaches the bound there each counts how many are larger.  Where too much does (rows of equal values) or too little (fewer than `top` values above
+// FLOOR), every value of the row is gone through again, each warp with its 32 best in registers.
+constexpr int UNROLL = 4, RESIDENT = 1024, TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
 
 template <int T> struct Shared {
     Part part[T / 32];
+    float high[32];                      // of the warps' threads, the 32 / (T / 32) largest of each
+    float block_high[32];                // of those the 32 / blocks largest
     Part block;                          // of this block, for the other blocks of the cluster
-    float bound[T / 32];
-    float block_bound;
     unsigned listed, found;
     unsigned list[LIST];
     unsigned long long key[CANDIDATES];
 };
-
-template <int T> __device__ __forceinline__ void team_sync() { if constexpr (T == 32) __syncwarp(); else __syncthreads(); }
+template <int T> __device__ __forceinline__ void team_sync() {
+    if constexpr (T == 32) __syncwarp();
+    else __syncthreads();
+}
+// The lane's place among the 32 lanes' values, of equal ones the lower lane first.
+__device__ __forceinline__ int place_in_warp(float v, unsigned lane) {
+    int place = 0;
+#pragma unroll
+    for (unsigned l = 0; l < 32u; ++l) {
+        const float other = __shfl_sync(ALL, v, l);
+        place += other > v || (other == v && l < lane) ? 1 : 0;
+    }
+    return place;
+}
 
 template <int TYPE, int T, bool MASKED, bool TOP>
-__global__ void __launch_bounds__(T == 32 ? 128 : T, T == 32 ? 6 : 4) k_long(Rows p, Outputs o, int blocks, int group) {
+__global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int blocks, int group) {
     using C = Chunk<TYPE>;
     using Value = typename Of<TYPE>::T;
-    constexpr int N = C::N, TEAMS = T == 32 ? 4 : 1, WARPS = T / 32;
-    extern __shared__ __align__(16) unsigned char shared_bytes[];
-    __shared__ Shared<T> shared_all[TEAMS];
-    const int team = T == 32 ? (int)threadIdx.x / 32 : 0, t = (int)threadIdx.x % T, warp = t / 32;
+    constexpr int N = C::N, WARPS = T / 32, BATCH = UNROLL * T;
+    static_assert(WARPS * 32 <= CANDIDATES, "the warps' best have to fit");
+    extern __shared__ __align__(128) unsigned char shared_bytes[];
+    __shared__ Shared<T> sh;
+    Value* const table = reinterpret_cast<Value*>(shared_bytes);
+    const int t = (int)threadIdx.x, warp = t / 32;
     const unsigned lane = threadIdx.x % 32u;
-    Shared<T>& sh = shared_all[team];
-    Value* table = reinterpret_cast<Value*>(shared_bytes) + team * (TABLE_ROWS + 1) * T;
-    const int rank = blocks > 1 ? (int)(blockIdx.x % (unsigned)blocks) : 0, threads = blocks * T, me = rank * T + t;
+    const int rank = blocks > 1 ? (int)(blockIdx.x % (unsigned)blocks) : 0;
     const float c = p.scale * LOG2E;
-    const long long first = (long long)(blockIdx.x / (unsigned)blocks) * TEAMS + team, step = (long long)(gridDim.x / (unsigned)blocks) * TEAMS;
+    const long long first = (long long)(blockIdx.x / (unsigned)blocks), step = gridDim.x / (unsigned)blocks;
+    cg::cluster_group cluster = cg::this_cluster();
     for (long long r = first; r < p.rows; r += step) {
         const Row<TYPE> row(p, r);
-        const int batches = (row.chunks + UNROLL * threads - 1) / (UNROLL * threads);
+        const int batches = (row.chunks + BATCH * blocks - 1) / (BATCH * blocks);      // of this block: the row's batch b * blocks + rank
         const int a = t == 0 && rank == 0 && p.taken ? __ldg(p.taken + r) : -1;
+        const bool has_end = rank == 0 && t < row.ends;                      // (ends < 2 N <= 16 <= T)
+        const float xe = has_end ? max_nan(row.at(row.end(t)), FLOOR) : FLOOR;
         Part part{FLOOR, 0.0f, 0.0f};
         Two s2 = two(0.0f, 0.0f), t2 = s2;
         float high = FLOOR;                                                  // of the group of batches
         for (int b = 0; b < batches; ++b) {
+            const int at = (b * blocks + rank) * BATCH + t;
             uint4 raw[UNROLL];
             unsigned legal[UNROLL][N / 4];
-            const int at = b * UNROLL * threads + me;
+            if constexpr (MASKED) {
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int k = at + u * threads;
-                raw[u] = k < row.chunks ? row.chunk(k) : C::fill();
-                if constexpr (MASKED) {
+                for (int u = 0; u < UNROLL; ++u) {
+                    const int k = at + u * T;
+#pragma unroll
+                    for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
                     if (k < row.chunks) mask_words<N>(row.legal, row.head + k * N, row.actions, legal[u]);
-                    else
-#pragma unroll
-                        for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
                 }
             }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) raw[u] = at + u * T < row.chunks ? row.chunk(at + u * T) : C::fill();
             float x[UNROLL][N], bm = FLOOR;
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 C::floored(raw[u], x[u]);
+                if constexpr (MASKED) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if constexpr (MASKED) x[u][i] = is_legal<N>(legal[u], i) ? x[u][i] : FLOOR;
-                    bm = fmaxf(bm, x[u][i]);
+                    for (int i = 0; i < N; ++i) x[u][i] = is_legal<N>(legal[u], i) ? x[u][i] : FLOOR;
                 }
+                largest<TYPE>(x[u], bm);
             }
             if constexpr (TOP) {
                 high = fmaxf(high, bm);
                 if ((b + 1) % group == 0 || b + 1 == batches) { table[(b / group) * T + t] = Of<TYPE>::put(high); high = FLOOR; }
             }
             if (bm > part.m) {
-                float u, v;
-                apart(s2, u, v); part.s += u + v; apart(t2, u, v); part.t += u + v;
+                part.s += sum2(s2); part.t += sum2(t2);
                 s2 = two(0.0f, 0.0f); t2 = s2;
                 rebase(part, bm, c);
             }
             const Two c2 = two(c, c), mc2 = two(-base_of(part.m, c), -base_of(part.m, c));
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-                for (int i = 0; i < N; i += 2) {
-                    const Two y2 = fma2(two(x[u][i], x[u][i + 1]), c2, mc2);
-                    float y0, y1;
-                    apart(y2, y0, y1);
-                    const Two e2 = two(exp2_fast(y0), exp2_fast(y1));
-                    s2 = add2(s2, e2);
-                    t2 = fma2(y2, e2, t2);
-                }
+            for (int u = 0; u < UNROLL; ++u) add_chunk<TYPE>(x[u], c2, mc2, s2, t2);
         }
-        { float u, v; apart(s2, u, v); part.s += u + v; apart(t2, u, v); part.t += u + v; }
-        const bool has_end = me < row.ends;                                  // (ends < 2 N <= 32 <= T: all in the first block)
-        const float xe = has_end ? max_nan(row.at(row.end(me)), FLOOR) : FLOOR;
+        part.s += sum2(s2); part.t += sum2(t2);
         if (has_end) take_one(part, xe, c);
         if constexpr (TOP) table[TABLE_ROWS * T + t] = Of<TYPE>::put(xe == xe ? xe : FLOOR);
         const float own = part.m;                                            // this thread's maximum
 
-        // join
-#pragma unroll
-        for (int by = 16; by; by /= 2) {
-            Part other;
-            other.m = __shfl_xor_sync(ALL, part.m, by); other.s = __shfl_xor_sync(ALL, part.s, by); other.t = __shfl_xor_sync(ALL, part.t, by);
-            join(part, other, c);
-        }
-        if constexpr (TOP) {                                                 // the warp's part of the bound
-            const int rank_wanted = (o.top + WARPS * blocks - 1) / (WARPS * blocks);
-            unsigned b = __float_as_uint(own);
-            b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
-            unsigned high_bits = 0u;
-            for (int k = 0; k < rank_wanted; ++k) {
-                high_bits = __reduce_max_sync(ALL, b);
-                const unsigned holders = __ballot_sync(ALL, b == high_bits);
-                if (lane == (unsigned)__ffs((int)holders) - 1u) b = 0u;
+        join_lanes(part, c);
+        if constexpr (TOP) {
+            if constexpr (WARPS > 1) {
+                constexpr int EACH = 32 / WARPS;
+                float v = own;
+                for (int k = 0; k < EACH; ++k) {
+                    const float largest_left = warp_max(v);
+                    if (lane == 0u) sh.high[warp * EACH + k] = largest_left;
+                    if (lane == (unsigned)__ffs((int)__ballot_sync(ALL, v == largest_left)) - 1u) v = NONE;
+                }
             }
-            if (lane == 0) sh.bound[warp] = high_bits == 0u ? FLOOR : __uint_as_float((high_bits & 0x80000000u) ? high_bits & 0x7FFFFFFFu : ~high_bits);
             if (t == 0) sh.listed = sh.found = 0u;
         }
-        if constexpr (T > 32) {
-            if (lane == 0) sh.part[warp] = part;
-            __syncthreads();
-            part = sh.part[0];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) join(part, sh.part[w], c);
-        } else __syncwarp();
+        if (lane == 0u) sh.part[warp] = part;
+        team_sync<T>();
         float bound = FLOOR;
-        if constexpr (TOP) {
-            bound = sh.bound[0];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) bound = fminf(bound, sh.bound[w]);
-        }
-        if constexpr (T > 32) {
-            if (blocks > 1) {
-                if (t == 0) { sh.block = part; sh.block_bound = bound; }
-                cg::cluster_group cluster = cg::this_cluster();
-                cluster.sync();
-                part = cluster.map_shared_rank(&sh, 0)->block;
-                for (int k = 1; k < blocks; ++k) join(part, cluster.map_shared_rank(&sh, k)->block, c);
-                if constexpr (TOP)
-                    for (int k = 0; k < blocks; ++k) bound = fminf(bound, cluster.map_shared_rank(&sh, k)->block_bound);
+        if constexpr (TOP) bound = WARPS > 1 ? sh.high[lane] : own;          // 32 values of the row, one a lane
+        if constexpr (T > 32) part = lane < WARPS ? sh.part[lane] : Part{FLOOR, 0.0f, 0.0f};
+        if (T > 32 && blocks > 1) {
+            if (warp == 0) {
+                if constexpr (TOP) sh.block_high[place_in_warp(bound, lane)] = bound;
+                join_lanes(part, c, WARPS);
+                if (lane == 0u) sh.block = part;
             }
+            cluster.sync();
+            const Shared<T>* const other = cluster.map_shared_rank(&sh, (int)(lane % (unsigned)blocks));
+            part = (int)lane < blocks ? other->block : Part{FLOOR, 0.0f, 0.0f};
+            if constexpr (TOP) bound = other->block_high[lane / (unsigned)blocks];
         }
-        if (!is_usual(part.m, c)) {
-            // beyond the limit: the maximum itself, then sums of exact differences; every block of a cluster goes through the whole row
-            float m = NONE;
-            for (int j = t; j < row.actions; j += T) m = fmaxf(m, row.at(j));
-#pragma unroll
-            for (int by = 16; by; by /= 2) m = fmaxf(m, __shfl_xor_sync(ALL, m, by));
+        if constexpr (TOP) bound = warp_min(place_in_warp(bound, lane) < o.top ? bound : INFINITY);
+        float m = warp_max(part.m);
+        if (is_usual(m, c)) {
+            if constexpr (T > 32) join_lanes(part, c, blocks > 1 ? 8 : WARPS);
+        } else {                                                             // beyond the limit; every block of a cluster goes through the whole row
+            m = exact_max(row, t, T);
             if constexpr (T > 32) {
-                __syncthreads();
-                if (lane == 0) sh.part[warp].m = m;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sh.part[w].m);
+                team_sync<T>();
+                if (lane == 0u) sh.part[warp].m = m;
+                team_sync<T>();
+                m = warp_max(sh.part[lane % WARPS].m);
             }
-            const float from = m == NONE ? 0.0f : m;
-            float s = 0.0f, sum = 0.0f;
-            for (int j = t; j < row.actions; j += T) {
-                const float y = (row.at(j) - from) * p.scale * LOG2E, e = exp2_fast(y);
-                s += e;
-                sum += e > 0.0f ? y * e : 0.0f;
-            }
-#pragma unroll
-            for (int by = 16; by; by /= 2) { s += __shfl_xor_sync(ALL, s, by); sum += __shfl_xor_sync(ALL, sum, by); }
-            part = Part{m, s, sum};
+            part = exact_sums(row, m, p.scale, t, T);
             if constexpr (T > 32) {
-                if (lane == 0) { sh.part[warp].s = s; sh.part[warp].t = sum; }
-                __syncthreads();
-                part.s = part.t = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) { part.s += sh.part[w].s; part.t += sh.part[w].t; }
+                team_sync<T>();
+                if (lane == 0u) sh.part[warp] = part;
+                team_sync<T>();
+                part = lane < WARPS ? sh.part[lane] : Part{m, 0.0f, 0.0f};
+                for (int by = WARPS / 2; by; by /= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
             }
         }
+        part.s = __shfl_sync(ALL, part.s, 0); part.t = __shfl_sync(ALL, part.t, 0); part.m = m;
         const Known known(part);
         if (t == 0 && rank == 0) {
             known.write(o, r);
             if (o.logprob) o.logprob[r] = known.bad ? known.log2_s : (unsigned)a >= (unsigned)row.actions ? 0.0f : known.logprob(row.at(a), p);
         }
         if constexpr (TOP) {
-            // batches that reach the bound, then what reaches it in them
+            // batches that reach the bound, then what reaches it in them: into the first block's list
+            Shared<T>* const to = T > 32 && blocks > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
             const int rows_used = (batches + group - 1) / group;
-            auto list_it = [&](int q) {
-                const unsigned place = atomicAdd(&sh.listed, 1u);
-                if (place < LIST) sh.list[place] = (unsigned)(q * T + t);
-            };
             if (bound > ABOVE_FLOOR && own >= bound) {
+                auto list_it = [&](int q) {
+                    const unsigned place = atomicAdd(&sh.listed, 1u);
+                    if (place < LIST) sh.list[place] = (unsigned)(q * T + t);
+                    else atomicAdd(&to->found, CANDIDATES + 1u);             // too many
+                };
                 for (int q = 0; q < rows_used; ++q)
                     if (Of<TYPE>::get(table[q * T + t]) >= bound) list_it(q);
                 if (xe >= bound) list_it(TABLE_ROWS);
             }
             team_sync<T>();
-            const unsigned listed = min(sh.listed, (unsigned)LIST);
-            for (unsigned l = (unsigned)warp; l < listed; l += WARPS) {
-                const int q = (int)sh.list[l] / T, owner = rank * T + (int)sh.list[l] % T;
-                const int values = q == TABLE_ROWS ? 1 : group * UNROLL * N;
-                for (int e = (int)lane; e < values; e += 32) {
-                    int j = -1;
-                    if (q == TABLE_ROWS) j = row.end(owner);
-                    else {
-                        const int k = (q * group * UNROLL + e / N) * threads + owner;
-                        if (k < row.chunks) j = row.head + k * N + e % N;
-                    }
-                    const float x = j >= 0 ? row.at(j) : NONE;
+            // a thread a chunk of a listed batch, so that all of them are read again at the same time
+            const int items = (int)min(sh.listed, (unsigned)LIST) * group * UNROLL;
+            for (int l = t; l < items; l += T) {
+                const int entry = (int)sh.list[l / (group * UNROLL)], q = entry / T, owner = entry % T, piece = l % (group * UNROLL);
+                auto take = [&](float x, int j) {
                     if (x >= bound) {
-                        const unsigned place = atomicAdd(&sh.found, 1u);
-                        if (place < CANDIDATES) sh.key[place] = order_key(x, (unsigned)j);
+                        const unsigned place = atomicAdd(&to->found, 1u);
+                        if (place < CANDIDATES) to->key[place] = order_key(x, (unsigned)j);
                     }
+                };
+                if (q == TABLE_ROWS) {
+                    if (piece == 0) take(row.at(row.end(owner)), row.end(owner));
+                    continue;
                 }
+                const int b = q * group + piece / UNROLL, k = (b * blocks + rank) * BATCH + piece % UNROLL * T + owner;
+                if (b >= batches || k >= row.chunks) continue;
+                float x[N];
+                C::floored(row.chunk(k), x);
+                if constexpr (MASKED) {
+                    unsigned legal[N / 4];
+                    mask_words<N>(row.legal, row.head + k * N, row.actions, legal);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) x[i] = is_legal<N>(legal, i) ? x[i] : FLOOR;
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) take(x[i], row.head + k * N + i);
             }
-            if (T > 32 && blocks > 1) cg::this_cluster().sync(); else team_sync<T>();
+            if (T > 32 && blocks > 1) cluster.sync(); else team_sync<T>();
             if (rank == 0) {
-                unsigned total = 0u;
-                bool over = !(bound > ABOVE_FLOOR);
-                for (int k = 0; k < blocks; ++k) {
-                    const Shared<T>* from = &sh;
-                    if constexpr (T > 32) if (blocks > 1) from = cg::this_cluster().map_shared_rank(&sh, k);
-                    total += from->found;
-                    over = over || from->listed > (unsigned)LIST || from->found > (unsigned)CANDIDATES;
-                }
-                over = over || total < (unsigned)o.top;
-                unsigned long long best = 0ull;
-                if (known.bad || known.nothing) {}
-                else if (!over) {
-                    if (warp == 0)
-                        for (int k = 0; k < blocks; ++k) {
-                            const Shared<T>* from = &sh;
-                            if constexpr (T > 32) if (blocks > 1) from = cg::this_cluster().map_shared_rank(&sh, k);
-                            const unsigned n = from->found;
-                            for (unsigned l = 0; l < n; l += 32u) take32(best, l + lane < n ? from->key[l + lane] : 0ull, lane, o.top);
-                        }
+                const unsigned n = sh.found;
+                if (n >= (unsigned)o.top && n <= (unsigned)CANDIDATES && !known.bad) {
+                    for (unsigned l = (unsigned)t; l < n; l += T) {
+                        const unsigned long long key = sh.key[l];
+                        const int place = place_of(key, sh.key, (int)n);
+                        if (place < o.top) write_top(o, p, known, r, place, key);
+                    }
                 } else {
-                    for (int j0 = warp * 32; j0 < row.actions; j0 += T) {
-                        const int j = j0 + (int)lane;
-                        const float x = j < row.actions ? row.at(j) : NONE;
-                        take32(best, x > NONE ? order_key(x, (unsigned)j) : 0ull, lane, o.top);
-                    }
+                    unsigned long long best = known.bad || known.nothing ? 0ull : best_of_all(row, warp * 32, T, lane, o.top);
                     if constexpr (T > 32) {
-                        __syncthreads();                                     // the keys of the short way have been counted by all
-                        if (WARPS * 32 <= CANDIDATES) sh.key[warp * 32 + lane] = best;
-                        __syncthreads();
-                        if (warp == 0)
-                            for (int w = 1; w < WARPS; ++w) best = merged32(best, sh.key[w * 32 + lane], lane);
+                        team_sync<T>();                                      // the list has been counted by all
+                        sh.key[t] = best;
+                        team_sync<T>();
                     }
-                }
-                if (warp == 0 && (int)lane < o.top) {
-                    o.top_actions[r * o.top + lane] = best ? key_action(best) : -1;
-                    o.top_logprobs[r * o.top + lane] = known.bad ? known.log2_s : best ? known.logprob(key_value(best), p) : NONE;
+                    if (warp == 0) {
+                        for (int w = 1; w < WARPS; ++w) best = merged32(best, sh.key[w * 32 + lane], lane);
+                        if ((int)lane < o.top) write_top(o, p, known, r, (int)lane, best);
+                    }
                 }
             }
         }
-        if (T > 32 && blocks > 1) cg::this_cluster().sync();                 // nobody leaves, or begins the next row, while its shared memory is read
-        else if constexpr (T > 32 || TOP) team_sync<T>();
+        if (T > 32 && blocks > 1) cluster.sync();                   // nobody leaves, or begins the next row, while its shared memory is read
+        else team_sync<T>();
     }
 }
 
@@ -611,104 +768,195 @@ struct Slope {
     }
 };
 
-template <int TYPE, int G, int E>
-__global__ void __launch_bounds__(256) k_short_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride, bool wide,
-                                                        bool wide_grad) {
+// Short rows have their sums in a few instructions: they are taken again instead of the statistics, which are as long as such a row.
+template <int TYPE, int G, int E, bool WIDE>
+__global__ void __launch_bounds__(256) k_short_backward(Rows p, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
     using O = Of<TYPE>;
-    const int lane = (int)threadIdx.x % G, j0 = lane * E;
+    const int lane = (int)threadIdx.x % G;
     const long long step = (long long)gridDim.x * (256 / G);
-    for (long long r = (long long)blockIdx.x * (256 / G) + (int)threadIdx.x / G; r < p.rows; r += step) {
-        float x[E];
-        load_short<TYPE, E>(p, r, j0, wide, x);
-        const Slope slope(p, stats, grad_logprob, grad_entropy, r);
-        unsigned bits = ~0u;
-        if (p.legal) mask_short<E>(p, r, j0, bits);
+    for (long long first = (long long)blockIdx.x * (256 / G); first < p.rows; first += step) {
+        const long long mine = first + (int)threadIdx.x / G, r = mine < p.rows ? mine : p.rows - 1;
+        float x[E], y[E], e[E];
+        load_short<TYPE, G, E, WIDE>(p, r, lane, x);
+        const int a = p.taken ? __ldg(p.taken + r) : -1;
+        const bool taken = (unsigned)a < (unsigned)p.actions;
+        const float gl = taken && grad_logprob ? __ldg(grad_logprob + r) : 0.0f, gh = grad_entropy ? __ldg(grad_entropy + r) : 0.0f;
+        const Part part = sum_short<G, E>(x, p.scale, y, e);
+        const Known known(part);
+        const float A = p.scale * (gl + gh * known.h), B = p.scale * gh * LN2, share = 1.0f / part.s;
+        float ya = FLOOR, ga = 0.0f;
+        int ia = -1;
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = bits >> i & 1u ? slope.one(x[i], j0 + i) : 0.0f;
-        auto* at = static_cast<typename O::T*>(grad) + r * grad_stride + j0;
-        if (wide_grad && j0 + E <= p.actions) {
-            constexpr int BYTES = E * (int)sizeof(typename O::T);
-            if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(at) = make_uint2(Chunk<TYPE>::two16(x[0], x[1]), Chunk<TYPE>::two16(x[2], x[3]));
-            else
+        for (int i = 0; i < E; ++i) {
+            const int j = short_action<G, E, WIDE>(lane, i);
+            if (taken && j == a) { ya = y[i]; ia = i; }
+            x[i] = x[i] == NONE || known.nothing ? 0.0f : -(e[i] * share) * fmaf(B, y[i] - known.log2_s, A);
+            if (known.bad) x[i] = known.log2_s;
+        }
+        if (ia >= 0) {
+            const float lp = (ya - known.log2_s) * LN2;
+            ga = p.scale * (-gl * expm1f(lp) - gh * exp2_fast(ya) * share * (lp + known.h));
+        }
+        const unsigned char* legal = p.legal ? p.legal + r * p.legal_stride : nullptr;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = short_action<G, E, WIDE>(lane, i);
+            if (i == ia && !known.nothing && !known.bad) x[i] = ga;
+            if (legal && j < p.actions && !__ldg(legal + j)) x[i] = 0.0f;
+        }
+        if (mine >= p.rows) continue;                                        // (a whole team: nothing of it is waited for)
+        auto* at = static_cast<typename O::T*>(grad) + r * grad_stride;
+        constexpr int BYTES = E * (int)sizeof(typename O::T);
+        if (WIDE && lane * E + E <= p.actions) {
+            if constexpr (BYTES == 8 && TYPE != CUDARL_F32) *reinterpret_cast<uint2*>(at + lane * E) = make_uint2(Chunk<TYPE>::two16(x[0], x[1]), Chunk<TYPE>::two16(x[2], x[3]));
+            else if constexpr (BYTES >= 16) {
 #pragma unroll
                 for (int k = 0; k < BYTES / 16; ++k) {
                     float part[Chunk<TYPE>::N];
 #pragma unroll
                     for (int i = 0; i < Chunk<TYPE>::N; ++i) part[i] = x[k * Chunk<TYPE>::N + i];
-                    reinterpret_cast<uint4*>(at)[k] = Chunk<TYPE>::pack(part);
+                    reinterpret_cast<uint4*>(at + lane * E)[k] = Chunk<TYPE>::pack(part);
                 }
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) if (j0 + i < p.actions) at[i] = O::put(x[i]);
+            for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions) at[j] = O::put(x[i]); }
         }
     }
 }
 
-// Long rows: T threads take UNROLL chunks each of a piece of a row; chunks begin where the gradient's address is aligned, and the logits are read in the same
-// chunks where their address is too, else one by one.
-template <int TYPE, int T, bool MASKED>
-__global__ void __launch_bounds__(256) k_long_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride, int pieces) {
+// A chunk's gradient.
+template <int TYPE>
+__device__ __forceinline__ void slope_chunk(const Slope& slope, bool usual, const uint4& raw, int j0, float (&v)[Chunk<TYPE>::N]) {
+    constexpr int N = Chunk<TYPE>::N;
+    if (usual && (unsigned)(slope.taken - j0) >= (unsigned)N) {
+        const Two c2 = two(slope.c, slope.c), mc2 = two(-slope.mc, -slope.mc), l2 = two(-slope.log2_s, -slope.log2_s), A2 = two(-slope.A, -slope.A), B2 = two(-slope.B, -slope.B);
+        Chunk<TYPE>::floored(raw, v);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const Two lp2 = add2(fma2(two(v[i], v[i + 1]), c2, mc2), l2);
+            float a, b;
+            apart(lp2, a, b);
+            apart(mul2(two(exp2_fast(a), exp2_fast(b)), fma2(B2, lp2, A2)), v[i], v[i + 1]);
+        }
+    } else {
+        Chunk<TYPE>::values(raw, v);
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            float one = v[0];
+#pragma unroll
+            for (int k = 1; k < N; ++k) one = i == k ? v[k] : one;
+            one = slope.one(one, j0 + i);
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = i == k ? one : v[k];
+        }
+    }
+}
+
+// A warp a row, all its chunks at once, the next row's on their way meanwhile.
+template <int TYPE, int CHUNKS, bool MASKED>
+__global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_warp_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad,
+                                                                                              long long grad_stride) {
     using C = Chunk<TYPE>;
     using O = Of<TYPE>;
-    constexpr int N = C::N, TEAMS = 256 / T;
-    const int team = (int)threadIdx.x / T, t = (int)threadIdx.x % T;
-    const long long work = p.rows * pieces, step = (long long)gridDim.x * TEAMS;
-    for (long long w = (long long)blockIdx.x * TEAMS + team; w < work; w += step) {
-        const long long r = pieces == 1 ? w : w / pieces;
-        const int piece = pieces == 1 ? 0 : (int)(w - r * pieces);
+    constexpr int N = C::N;
+    const int lane = (int)threadIdx.x % 32;
+    const long long step = (long long)gridDim.x * 8;
+    uint4 raw[CHUNKS];
+    typename O::T end;
+    struct Place { const typename O::T* x; typename O::T* g; const unsigned char* legal; int head, chunks, ends; };
+    auto place = [&](long long r) {
+        Place w;
+        w.x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
+        w.g = static_cast<typename O::T*>(grad) + r * grad_stride;
+        w.legal = MASKED ? p.legal + r * p.legal_stride : nullptr;
+        w.head = min((int)((16u - ((unsigned)reinterpret_cast<uintptr_t>(w.g) & 15u)) & 15u) / (int)sizeof(typename O::T), p.actions);
+        w.chunks = (p.actions - w.head) / N;
+        w.ends = p.actions - w.chunks * N;
+        return w;
+    };
+    auto load = [&](const Place& w) {
+        const bool together = (((unsigned)reinterpret_cast<uintptr_t>(w.x) ^ (unsigned)reinterpret_cast<uintptr_t>(w.g)) & 15u) == 0u;
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            const int k = lane + 32 * u;
+            raw[u] = C::fill();
+            if (k < w.chunks) raw[u] = together ? *reinterpret_cast<const uint4*>(w.x + w.head + k * N) : gather_chunk(w.x + w.head + k * N);
+        }
+        if (lane < w.ends) end = w.x[lane < w.head ? lane : w.chunks * N + lane];
+    };
+    long long r = (long long)blockIdx.x * 8 + (int)threadIdx.x / 32;
+    if (r < p.rows) load(place(r));
+    for (; r < p.rows; r += step) {
+        const Place w = place(r);
+        const Slope slope(p, stats, grad_logprob, grad_entropy, r);
+        const bool usual = slope.usual();
+        float v[CHUNKS][N];
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) slope_chunk<TYPE>(slope, usual, raw[u], w.head + (lane + 32 * u) * N, v[u]);
+        const int je = lane < w.head ? lane : w.chunks * N + lane;
+        const float ve = lane < w.ends ? slope.one(O::get(end), je) : 0.0f;
+        if (r + step < p.rows) load(place(r + step));                        // (another row: what is written below is not read there)
+#pragma unroll
+        for (int u = 0; u < CHUNKS; ++u) {
+            const int k = lane + 32 * u;
+            if (k >= w.chunks) continue;
+            if constexpr (MASKED) {
+                unsigned mask[N / 4];
+                mask_words<N>(w.legal, w.head + k * N, p.actions, mask);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[u][i] = is_legal<N>(mask, i) ? v[u][i] : 0.0f;
+            }
+            *reinterpret_cast<uint4*>(w.g + w.head + k * N) = C::pack(v[u]);
+        }
+        if (lane < w.ends) w.g[je] = O::put(MASKED && !__ldg(w.legal + je) ? 0.0f : ve);
+    }
+}
+
+// Long rows: a block takes UNROLL chunks a thread of a piece of a row; chunks begin where the gradient's address is aligned, and the logits are read in the same
+// chunks where their address is too, else one by one.
+template <int TYPE, bool MASKED>
+__global__ void __launch_bounds__(256) k_long_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
+    using C = Chunk<TYPE>;
+    using O = Of<TYPE>;
+    constexpr int N = C::N, T = 256;
+    const int t = (int)threadIdx.x;
+    for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const auto* x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
         auto* g = static_cast<typename O::T*>(grad) + r * grad_stride;
         const unsigned char* legal = MASKED ? p.legal + r * p.legal_stride : nullptr;
         const int head = min((int)((16u - ((unsigned)reinterpret_cast<uintptr_t>(g) & 15u)) & 15u) / (int)sizeof(typename O::T), p.actions);
         const int chunks = (p.actions - head) / N, ends = p.actions - chunks * N;
         const bool together = (((unsigned)reinterpret_cast<uintptr_t>(x) ^ (unsigned)reinterpret_cast<uintptr_t>(g)) & 15u) == 0u;
+        const int base = (int)blockIdx.x * UNROLL * T + t;
+        uint4 raw[UNROLL];
+        unsigned mask[UNROLL][N / 4];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = base + u * T;
+            raw[u] = C::fill();
+            if (k < chunks) {
+                raw[u] = together ? *reinterpret_cast<const uint4*>(x + head + k * N) : gather_chunk(x + head + k * N);
+                if constexpr (MASKED) mask_words<N>(legal, head + k * N, p.actions, mask[u]);
+            }
+        }
         const Slope slope(p, stats, grad_logprob, grad_entropy, r);
-        if (piece == 0 && t < ends) {
+        const bool usual = slope.usual();
+        if (blockIdx.x == 0u && t < ends) {
             const int j = t < head ? t : chunks * N + t;
             g[j] = O::put(MASKED && !__ldg(legal + j) ? 0.0f : slope.one(O::get(x[j]), j));
         }
-        const bool usual = slope.usual();
-        const Two c2 = two(slope.c, slope.c), mc2 = two(-slope.mc, -slope.mc), l2 = two(-slope.log2_s, -slope.log2_s), A2 = two(slope.A, slope.A), B2 = two(slope.B, slope.B),
-                  minus = two(-1.0f, -1.0f);
-        for (int base = piece * UNROLL * T; base < chunks; base += pieces * UNROLL * T) {
-            uint4 raw[UNROLL];
-            unsigned mask[UNROLL][N / 4];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int k = base + u * T + t;
-                raw[u] = C::fill();
-                if (k < chunks) {
-                    const auto* at = x + head + k * N;
-                    if (together) raw[u] = *reinterpret_cast<const uint4*>(at);
-                    else raw[u] = gather_chunk(at);
-                    if constexpr (MASKED) mask_words<N>(legal, head + k * N, p.actions, mask[u]);
-                }
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = base + u * T;
+            if (k >= chunks) continue;
+            float v[N];
+            slope_chunk<TYPE>(slope, usual, raw[u], head + k * N, v);
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = is_legal<N>(mask[u], i) ? v[i] : 0.0f;
             }
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const int k = base + u * T + t;
-                if (k >= chunks) continue;
-                float v[N];
-                const int j0 = head + k * N;
-                if (usual && (unsigned)(slope.taken - j0) >= (unsigned)N) {
-                    C::floored(raw[u], v);
-#pragma unroll
-                    for (int i = 0; i < N; i += 2) {
-                        const Two lp2 = add2(fma2(two(v[i], v[i + 1]), c2, mc2), l2);
-                        float a, b;
-                        apart(lp2, a, b);
-                        apart(mul2(mul2(two(exp2_fast(a), exp2_fast(b)), minus), fma2(B2, lp2, A2)), v[i], v[i + 1]);
-                    }
-                } else {
-                    C::values(raw[u], v);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) v[i] = slope.one(v[i], j0 + i);
-                }
-                if constexpr (MASKED)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) v[i] = is_legal<N>(mask[u], i) ? v[i] : 0.0f;
-                *reinterpret_cast<uint4*>(g + j0) = C::pack(v);
-            }
+            *reinterpret_cast<uint4*>(g + head + k * N) = C::pack(v);
         }
     }
 }
@@ -740,30 +988,65 @@ bool aligned_rows(const void* base, long long stride, int value, int bytes) {
     return reinterpret_cast<uintptr_t>(base) % (unsigned)bytes == 0 && stride * value % bytes == 0;
 }
 
-constexpr int SHORT_ACTIONS = 128, WARP_ACTIONS = 2048;
+constexpr int SHORT_ACTIONS = 128, WARP_ACTIONS = 1024;
 
-template <int TYPE, int G, int E>
+template <int TYPE, int G, int E, bool WIDE>
 cudaError_t launch_short(const Rows& p, const Outputs& o, cudaStream_t st) {
-    constexpr int value = (int)sizeof(typename Of<TYPE>::T), bytes = E * value < 16 ? E * value : 16;
-    const bool wide = aligned_rows(p.logits, p.stride, value, bytes);
     const unsigned grid = blocks_of(p.rows, 256 / G);
-    if (o.top) k_short<TYPE, G, E, true><<<grid, 256, 0, st>>>(p, o, wide);
-    else k_short<TYPE, G, E, false><<<grid, 256, 0, st>>>(p, o, wide);
+    if (o.top) k_short<TYPE, G, E, WIDE, true><<<grid, 256, 0, st>>>(p, o);
+    else k_short<TYPE, G, E, WIDE, false><<<grid, 256, 0, st>>>(p, o);
+    return cudaGetLastError();
+}
+struct BackwardArgs { const float4* stats; const float* gl; const float* gh; void* grad; long long stride; };
+template <int TYPE, int G, int E, bool WIDE>
+cudaError_t launch_short(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
+    k_short_backward<TYPE, G, E, WIDE><<<blocks_of(p.rows, 256 / G), 256, 0, st>>>(p, b.gl, b.gh, b.grad, b.stride);
+    return cudaGetLastError();
+}
+// Rows of up to SHORT_ACTIONS actions, either way (a call's outputs or a gradient's arguments).
+template <int TYPE, class Args>
+cudaError_t launch_short(const Rows& p, const Args& args, bool wide4, bool wide8, cudaStream_t st) {
+    const int v = p.actions;
+    if (v <= 4 && wide4) return launch_short<TYPE, 1, 4, true>(p, args, st);
+    if (v <= 8) return wide8 ? launch_short<TYPE, 1, 8, true>(p, args, st) : launch_short<TYPE, 4, 2, false>(p, args, st);
+    if (v <= 16) return wide8 ? launch_short<TYPE, 2, 8, true>(p, args, st) : launch_short<TYPE, 4, 4, false>(p, args, st);
+    if (v <= 32) return wide8 ? launch_short<TYPE, 4, 8, true>(p, args, st) : launch_short<TYPE, 4, 8, false>(p, args, st);
+    if (v <= 64) return wide8 ? launch_short<TYPE, 8, 8, true>(p, args, st) : launch_short<TYPE, 8, 8, false>(p, args, st);
+    return wide8 ? launch_short<TYPE, 16, 8, true>(p, args, st) : launch_short<TYPE, 16, 8, false>(p, args, st);
+}
+
+template <int TYPE, int VALUES>
+cudaError_t launch_warp(const Rows& p, const Outputs& o, int sms, cudaStream_t st) {
+    constexpr int CHUNKS = VALUES / 32 / Chunk<TYPE>::N;
+    const unsigned most = (unsigned)(sms * warp_blocks(VALUES / 32)), all = blocks_of(p.rows, 8), grid = all < most ? all : most;
+    if (p.legal) {
+        if (o.top) k_warp<TYPE, CHUNKS, true, true><<<grid, 256, 0, st>>>(p, o);
+        else k_warp<TYPE, CHUNKS, true, false><<<grid, 256, 0, st>>>(p, o);
+    } else {
+        if (o.top) k_warp<TYPE, CHUNKS, false, true><<<grid, 256, 0, st>>>(p, o);
+        else k_warp<TYPE, CHUNKS, false, false><<<grid, 256, 0, st>>>(p, o);
+    }
+    return cudaGetLastError();
+}
+template <int TYPE, int VALUES>
+cudaError_t launch_warp(const Rows& p, const BackwardArgs& b, int sms, cudaStream_t st) {
+    constexpr int CHUNKS = VALUES / 32 / Chunk<TYPE>::N;
+    const unsigned most = (unsigned)(sms * warp_blocks(VALUES / 32)), all = blocks_of(p.rows, 8), grid = all < most ? all : most;
+    if (p.legal) k_warp_backward<TYPE, CHUNKS, true><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
+    else k_warp_backward<TYPE, CHUNKS, false><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
     return cudaGetLastError();
 }
 
 template <int TYPE, int T, bool MASKED, bool TOP>
-cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, cudaStream_t st) {
-    constexpr int TEAMS = T == 32 ? 4 : 1, N = Chunk<TYPE>::N;
-    const long long batches = ((long long)p.actions / N + UNROLL * (long long)T * blocks - 1) / (UNROLL * (long long)T * blocks);
-    const int group = (int)((batches + TABLE_ROWS - 1) / TABLE_ROWS > 1 ? (batches + TABLE_ROWS - 1) / TABLE_ROWS : 1);
-    const size_t table = TOP ? (size_t)(TABLE_ROWS + 1) * T * TEAMS * sizeof(typename Of<TYPE>::T) : 0;
+cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, int sms, cudaStream_t st) {
+    const long long batch = (long long)UNROLL * T * blocks, chunks = p.actions / Chunk<TYPE>::N;
+    const int group = (int)((chunks + batch * TABLE_ROWS) / (batch * TABLE_ROWS));
+    const long long resident = (long long)sms * (RESIDENT / T);
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(T == 32 ? 128 : T);
-    cfg.dynamicSmemBytes = table;
+    cfg.blockDim = dim3(T);
+    cfg.dynamicSmemBytes = TOP ? (size_t)(TABLE_ROWS + 1) * T * sizeof(typename Of<TYPE>::T) : 0;
     cfg.stream = st;
-    const unsigned teams = blocks_of(p.rows, TEAMS);
-    cfg.gridDim = dim3((teams < 1u << 24 ? teams : 1u << 24) * (unsigned)blocks);
+    cfg.gridDim = dim3((unsigned)((p.rows > resident ? resident : p.rows) * blocks));
     cudaLaunchAttribute attr[1];
     if (blocks > 1) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -773,56 +1056,46 @@ cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, cudaStream_
     return cudaLaunchKernelEx(&cfg, k_long<TYPE, T, MASKED, TOP>, p, o, blocks, group);
 }
 template <int TYPE, int T>
-cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, cudaStream_t st) {
-    if (p.legal) return o.top ? launch_long<TYPE, T, true, true>(p, o, blocks, st) : launch_long<TYPE, T, true, false>(p, o, blocks, st);
-    return o.top ? launch_long<TYPE, T, false, true>(p, o, blocks, st) : launch_long<TYPE, T, false, false>(p, o, blocks, st);
+cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, int sms, cudaStream_t st) {
+    if (p.legal) return o.top ? launch_long<TYPE, T, true, true>(p, o, blocks, sms, st) : launch_long<TYPE, T, true, false>(p, o, blocks, sms, st);
+    return o.top ? launch_long<TYPE, T, false, true>(p, o, blocks, sms, st) : launch_long<TYPE, T, false, false>(p, o, blocks, sms, st);
 }
 
 template <int TYPE>
 cudaError_t launch_rows(const Rows& p, const Outputs& o, int sms, cudaStream_t st) {
+    constexpr int value = (int)sizeof(typename Of<TYPE>::T);
     const int v = p.actions;
-    if (v <= 4) return launch_short<TYPE, 1, 4>(p, o, st);
-    if (v <= 8) return launch_short<TYPE, 1, 8>(p, o, st);
-    if (v <= 16) return launch_short<TYPE, 2, 8>(p, o, st);
-    if (v <= 32) return launch_short<TYPE, 4, 8>(p, o, st);
-    if (v <= 64) return launch_short<TYPE, 8, 8>(p, o, st);
-    if (v <= SHORT_ACTIONS) return launch_short<TYPE, 16, 8>(p, o, st);
-    if (v <= WARP_ACTIONS) return launch_long<TYPE, 32>(p, o, 1, st);
+    if (v <= SHORT_ACTIONS) return launch_short<TYPE>(p, o, aligned_rows(p.logits, p.stride, value, 4 * value), aligned_rows(p.logits, p.stride, value, 16), st);
+    if (v <= 256) return launch_warp<TYPE, 256>(p, o, sms, st);
+    if (v <= 512) return launch_warp<TYPE, 512>(p, o, sms, st);
+    if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, o, sms, st);
     // a cluster for each row where there are too few rows to occupy the GPU, as long as each block still gets half a batch
     int blocks = 1;
     while (blocks < 8 && p.rows * blocks * 2 <= sms * 2 && (long long)v >= 256ll * Chunk<TYPE>::N * UNROLL / 2 * blocks * 2) blocks *= 2;
-    return launch_long<TYPE, 256>(p, o, blocks, st);
+    if (const char* e = getenv("POLICY_BLOCKS")) blocks = atoi(e);
+    const char* e = getenv("POLICY_T");
+    const int T = e ? atoi(e) : 256;
+    if (T == 32) return launch_long<TYPE, 32>(p, o, 1, sms, st);
+    if (T == 64) return launch_long<TYPE, 64>(p, o, blocks, sms, st);
+    if (T == 128) return launch_long<TYPE, 128>(p, o, blocks, sms, st);
+    return launch_long<TYPE, 256>(p, o, blocks, sms, st);
 }
 
-struct BackwardArgs { const float4* stats; const float* gl; const float* gh; void* grad; long long stride; };
-
-template <int TYPE, int G, int E>
-cudaError_t launch_short_backward(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
-    constexpr int value = (int)sizeof(typename Of<TYPE>::T), bytes = E * value < 16 ? E * value : 16;
-    k_short_backward<TYPE, G, E><<<blocks_of(p.rows, 256 / G), 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride, aligned_rows(p.logits, p.stride, value, bytes),
-                                                                             aligned_rows(b.grad, b.stride, value, bytes));
-    return cudaGetLastError();
-}
-template <int TYPE, int T>
-cudaError_t launch_long_backward(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
-    const long long each = (long long)T * UNROLL * Chunk<TYPE>::N;
-    const int pieces = T == 32 ? 1 : (int)((p.actions + each - 1) / each);
-    const unsigned grid = p.rows > (1ll << 50) / pieces ? 1u << 28 : blocks_of(p.rows * pieces, 256 / T);
-    if (p.legal) k_long_backward<TYPE, T, true><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride, pieces);
-    else k_long_backward<TYPE, T, false><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride, pieces);
-    return cudaGetLastError();
-}
 template <int TYPE>
-cudaError_t launch_backward(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
+cudaError_t launch_backward(const Rows& p, const BackwardArgs& b, int sms, cudaStream_t st) {
+    constexpr int value = (int)sizeof(typename Of<TYPE>::T);
     const int v = p.actions;
-    if (v <= 4) return launch_short_backward<TYPE, 1, 4>(p, b, st);
-    if (v <= 8) return launch_short_backward<TYPE, 1, 8>(p, b, st);
-    if (v <= 16) return launch_short_backward<TYPE, 2, 8>(p, b, st);
-    if (v <= 32) return launch_short_backward<TYPE, 4, 8>(p, b, st);
-    if (v <= 64) return launch_short_backward<TYPE, 8, 8>(p, b, st);
-    if (v <= SHORT_ACTIONS) return launch_short_backward<TYPE, 16, 8>(p, b, st);
-    if (v <= WARP_ACTIONS) return launch_long_backward<TYPE, 32>(p, b, st);
-    return launch_long_backward<TYPE, 256>(p, b, st);
+    if (v <= SHORT_ACTIONS)
+        return launch_short<TYPE>(p, b, aligned_rows(p.logits, p.stride, value, 4 * value) && aligned_rows(b.grad, b.stride, value, 4 * value),
+                                  aligned_rows(p.logits, p.stride, value, 16) && aligned_rows(b.grad, b.stride, value, 16), st);
+    if (v <= 256) return launch_warp<TYPE, 256>(p, b, sms, st);
+    if (v <= 512) return launch_warp<TYPE, 512>(p, b, sms, st);
+    if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, b, sms, st);
+    const int each = 256 * UNROLL * Chunk<TYPE>::N;
+    const dim3 grid((unsigned)((v + each - 1) / each), (unsigned)(p.rows < 65535 ? p.rows : 65535));
+    if (p.legal) k_long_backward<TYPE, true><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
+    else k_long_backward<TYPE, false><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -867,11 +1140,13 @@ extern "C" int cudarl_policy_logprobs_backward(const cudarl_policy_rows* p, cons
         (rc = arrays.check("stats", stats, 16)) || (rc = arrays.check_if("grad_logprob", grad_logprob, 4)) || (rc = arrays.check_if("grad_entropy", grad_entropy, 4)) ||
         (rc = arrays.check("grad_logits", grad_logits, align))) return rc;
     CurrentDevice current;
+    int sms = 0;
     cudaError_t e = current.set(arrays.device());
-    if (e != cudaSuccess) return fail_cuda("cudaSetDevice", e);
+    if (e == cudaSuccess) e = multiprocessors(&sms);
+    if (e != cudaSuccess) return fail_cuda("cudarl_policy_logprobs_backward", e);
     const Rows r = device_rows(p);
     const BackwardArgs b{reinterpret_cast<const float4*>(stats), grad_logprob, grad_entropy, grad_logits, (long long)grad_stride};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    e = p->type == CUDARL_F32 ? launch_backward<CUDARL_F32>(r, b, st) : p->type == CUDARL_BF16 ? launch_backward<CUDARL_BF16>(r, b, st) : launch_backward<CUDARL_F16>(r, b, st);
+    e = p->type == CUDARL_F32 ? launch_backward<CUDARL_F32>(r, b, sms, st) : p->type == CUDARL_BF16 ? launch_backward<CUDARL_BF16>(r, b, sms, st) : launch_backward<CUDARL_F16>(r, b, sms, st);
     return e == cudaSuccess ? 0 : fail_cuda("cudarl_policy_logprobs_backward", e);
 }
