@@ -44,6 +44,7 @@ struct Control {
 
 struct Settings {
     float beta1, rest1, beta2, rest2, eps;    // rest = 1 - beta
+    float one;                                // 1
     unsigned keys[20];                        // of the ten Philox rounds
     int clipped;
     double power1, power2;                    // the betas
@@ -410,11 +411,12 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
             }
         }
         float root[8];
+        const Two one2 = two(s.one, s.one);                                  // (a product by a one that the compiler does not know, plus: a sum that it cannot fuse with the product before)
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             const Two gi = mul2(two(g[i], g[i + 1]), two(scale, scale));
-            const Two mi = add2(mul2(two(s.beta1, s.beta1), two(m[i], m[i + 1])), mul2(two(s.rest1, s.rest1), gi));
-            const Two vi = add2(mul2(two(s.beta2, s.beta2), two(v[i], v[i + 1])), mul2(mul2(two(s.rest2, s.rest2), gi), gi)), ri = root2(vi);
+            const Two mi = fma2(mul2(two(s.beta1, s.beta1), two(m[i], m[i + 1])), one2, mul2(two(s.rest1, s.rest1), gi));
+            const Two vi = fma2(mul2(two(s.beta2, s.beta2), two(v[i], v[i + 1])), one2, mul2(mul2(two(s.rest2, s.rest2), gi), gi)), ri = root2(vi);
             float a, b;
             apart(fma2(ri, two(root_fix2, root_fix2), two(s.eps, s.eps)), a, b);
             const Two wi = two(w[i], w[i + 1]), way = mul2(mul2(mi, two(fix1, fix1)), two(reciprocal_fast(a), reciprocal_fast(b)));
@@ -619,7 +621,7 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
     if (e != cudaSuccess) return fail_cuda("cudaSetDevice", e);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudarl_adamw_config& c = o->cfg;
-    Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, {}, c.max_grad_norm > 0.0f, c.beta1, c.beta2};
+    Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, 1.0f, {}, c.max_grad_norm > 0.0f, c.beta1, c.beta2};
     for (unsigned r = 0; r < 10; ++r) {
         s.keys[2 * r] = (unsigned)c.seed + r * 0x9E3779B9u;
         s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;

@@ -89,7 +89,7 @@ template <> struct Of<CUDARL_F16> {
     static __device__ __forceinline__ T put(float v) { return __float2half_rn(v); }
 };
 
-// Two floats for the instructions that take two: half as many to issue, each of the two rounded as by itself.
+// Two floats for the instructions that take two: half as many to issue, each of the two rounded as by itself.  (mul2 into add2 may become one fma2.)
 typedef unsigned long long Two;
 __device__ __forceinline__ Two two(float a, float b) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void apart(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }

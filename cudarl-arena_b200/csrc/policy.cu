@@ -10,7 +10,6 @@
 // test.  Rows with |m c| of 2^23 and more, where the error would be whole powers of two, are gone through a second time with exact differences.
 #include "caller_arrays.cuh"
 #include <cooperative_groups.h>
-#include <cstdlib>
 
 namespace {
 using namespace cudarl;
@@ -37,6 +36,8 @@ struct Outputs {
 __device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float sum2(Two v) { float a, b; apart(v, a, b); return a + b; }
+
 // Larger for the larger logit, of equal ones for the lower action; 0 for none.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned action) {
     const unsigned b = __float_as_uint(x + 0.0f);                            // -0 counts as 0
@@ -61,7 +62,7 @@ __device__ __forceinline__ void rebase(Part& p, float m, float c) {          // 
 }
 __device__ __forceinline__ void take_one(Part& p, float x, float c) {
     if (x > p.m) rebase(p, x, c);
-    const float y = fmaf(x, c, -base_of(p.m, c)), e = exp2_fast(y);
+    const float y = fmaf(max_nan(x, FLOOR), c, -base_of(p.m, c)), e = exp2_fast(y);
     p.s += e;
     p.t = fmaf(y, e, p.t);
 }
@@ -71,7 +72,7 @@ struct Known {
     bool nothing, bad;                                                       // no action has any probability; a NaN or plus infinity is among them
     __device__ __forceinline__ Known(const Part& p) {
         nothing = p.s == 0.0f; bad = !(p.s == p.s);
-        m = p.m; log2_s = log2f(p.s); h = nothing ? 0.0f : LN2 * (log2_s - p.t / p.s);
+        m = p.m; log2_s = __log2f(p.s); h = nothing ? 0.0f : LN2 * (log2_s - __fdividef(p.t, p.s));      // (s is 1 or more: both are good to some 2^-22)
     }
     // Log probability of an action with this logit.
     __device__ __forceinline__ float logprob(float x, const Rows& p) const {
@@ -94,7 +95,7 @@ template <> struct Chunk<CUDARL_F32> {
     static __device__ __forceinline__ void values(const uint4& v, float (&x)[4]) {
         x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
-    static __device__ __forceinline__ uint4 fill() { const unsigned f = __float_as_uint(FLOOR); return make_uint4(f, f, f, f); }
+    static __device__ __forceinline__ uint4 fill() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }                // minus infinities
     static __device__ __forceinline__ void floored(const uint4& v, float (&x)[4]) {
         values(v, x);
 #pragma unroll
@@ -107,7 +108,7 @@ template <> struct Chunk<CUDARL_BF16> {
     static constexpr unsigned FLOOR2 = 0xE0ADE0ADu;                          // FLOOR, rounded to bf16, twice
     static __device__ __forceinline__ void pair(unsigned v, float& a, float& b) { a = __uint_as_float(v << 16); b = __uint_as_float(v & 0xFFFF0000u); }
     static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) { pair(v.x, x[0], x[1]); pair(v.y, x[2], x[3]); pair(v.z, x[4], x[5]); pair(v.w, x[6], x[7]); }
-    static __device__ __forceinline__ uint4 fill() { return make_uint4(FLOOR2, FLOOR2, FLOOR2, FLOOR2); }
+    static __device__ __forceinline__ uint4 fill() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
     static __device__ __forceinline__ unsigned up(unsigned v) { unsigned r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(FLOOR2)); return r; }
     static __device__ __forceinline__ void floored(const uint4& v, float (&x)[8]) { values(make_uint4(up(v.x), up(v.y), up(v.z), up(v.w)), x); }
     static __device__ __forceinline__ unsigned two16(float a, float b) { const __nv_bfloat162 v = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const unsigned*>(&v); }
@@ -117,7 +118,7 @@ template <> struct Chunk<CUDARL_F16> {
     static constexpr int N = 8;
     static __device__ __forceinline__ void pair(unsigned v, float& a, float& b) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v)); a = f.x; b = f.y; }
     static __device__ __forceinline__ void values(const uint4& v, float (&x)[8]) { pair(v.x, x[0], x[1]); pair(v.y, x[2], x[3]); pair(v.z, x[4], x[5]); pair(v.w, x[6], x[7]); }
-    static __device__ __forceinline__ uint4 fill() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }      // minus infinity: FLOOR is not an f16
+    static __device__ __forceinline__ uint4 fill() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
     static __device__ __forceinline__ void floored(const uint4& v, float (&x)[8]) {
         values(v, x);
 #pragma unroll
@@ -172,6 +173,10 @@ struct Row {
         head = min((int)((16u - ((unsigned)reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / (int)sizeof(typename O::T), actions);
         chunks = (actions - head) / N;
         ends = actions - chunks * N;
+    }
+    __device__ __forceinline__ void move_to(const Rows& p, long long r) {    // to another row that lies as this one does to 16 bytes
+        x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
+        if (legal) legal = p.legal + r * p.legal_stride;
     }
     __device__ __forceinline__ float at(int j) const { return legal && !__ldg(legal + j) ? NONE : O::get(x[j]); }
     __device__ __forceinline__ int end(int i) const { return i < head ? i : chunks * N + i; }       // the action of the i-th of the ends
@@ -245,25 +250,32 @@ __device__ __forceinline__ void load_short(const Rows& p, long long r, int lane,
     }
 }
 
-// y and 2^y of the lane's values, and the row's part in all its lanes.
+// y and 2^y of the lane's values, and the row's part in all its lanes.  `exact`: the row is beyond the limit.
 template <int G, int E>
-__device__ __forceinline__ Part sum_short(const float (&x)[E], float scale, float (&y)[E], float (&e)[E]) {
+__device__ __forceinline__ Part sum_short(const float (&x)[E], float scale, float (&y)[E], float (&e)[E], bool& exact) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < E; ++i) m = fmaxf(m, x[i]);
 #pragma unroll
     for (int by = 1; by < G; by *= 2) m = fmaxf(m, __shfl_xor_sync(ALL, m, by));
-    const float c = scale * LOG2E, mc = m * c, from = m == NONE ? 0.0f : m;
-    const bool exact = !is_usual(m, c);
-    Part part{m, 0.0f, 0.0f};
+    const float c = scale * LOG2E, mc = m * c;
+    exact = !is_usual(m, c);
+    const Two c2 = two(c, c), mc2 = two(-mc, -mc);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        y[i] = fmaf(max_nan(x[i], FLOOR), c, -mc);
-        if (exact) y[i] = max_nan((x[i] - from) * scale * LOG2E, FLOOR);
-        e[i] = exp2_fast(y[i]);
-        part.s += e[i];
-        part.t = fmaf(y[i], e[i], part.t);
+    for (int i = 0; i < E; i += 2) apart(fma2(two(max_nan(x[i], FLOOR), max_nan(x[i + 1], FLOOR)), c2, mc2), y[i], y[i + 1]);
+    if (__any_sync(ALL, exact)) {
+        const float from = m == NONE ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = exact ? max_nan((x[i] - from) * scale * LOG2E, FLOOR) : y[i];
     }
+    Two s2 = two(0.0f, 0.0f), t2 = s2;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        e[i] = exp2_fast(y[i]); e[i + 1] = exp2_fast(y[i + 1]);
+        s2 = add2(s2, two(e[i], e[i + 1]));
+        t2 = fma2(two(y[i], y[i + 1]), two(e[i], e[i + 1]), t2);
+    }
+    Part part{m, sum2(s2), sum2(t2)};
 #pragma unroll
     for (int by = 1; by < G; by *= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
     return part;
@@ -280,46 +292,45 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
         float x[E], y[E], e[E];
         load_short<TYPE, G, E, WIDE>(p, r, lane, x);
         const int a = p.taken ? __ldg(p.taken + r) : -1;
-        const Known known(sum_short<G, E>(x, p.scale, y, e));
+        bool exact;
+        const Known known(sum_short<G, E>(x, p.scale, y, e, exact));
         if (write) {
             if (lane == 0 && o.entropy) o.entropy[r] = known.h;
             if (o.logprob) {
-                if ((unsigned)a >= (unsigned)p.actions) { if (lane == 0) o.logprob[r] = known.bad ? known.log2_s : 0.0f; }
-                else {
-                    float xa = x[0];
-                    bool has = a == short_action<G, E, WIDE>(lane, 0);
+                float xa = x[0], ya = y[0];
+                bool has = a == short_action<G, E, WIDE>(lane, 0);
 #pragma unroll
-                    for (int i = 1; i < E; ++i) { const bool is = a == short_action<G, E, WIDE>(lane, i); xa = is ? x[i] : xa; has = has || is; }
-                    if (has) o.logprob[r] = known.logprob(xa, p);            // the lane that holds it
-                }
+                for (int i = 1; i < E; ++i) { const bool is = a == short_action<G, E, WIDE>(lane, i); xa = is ? x[i] : xa; ya = is ? y[i] : ya; has = has || is; }
+                const bool none = (unsigned)a >= (unsigned)p.actions;        // (then no lane holds it: the first writes)
+                float lp = LN2 * (ya - known.log2_s);
+                if (exact || known.bad || xa < -LARGE) lp = known.logprob(xa, p);
+                if (none) lp = known.bad ? known.log2_s : 0.0f;
+                if (none ? lane == 0 : has) o.logprob[r] = lp;
             }
         }
         if constexpr (TOP) {
-            // every lane's own values in falling order, then the largest head of the G lists, `top` times
-            unsigned long long key[E];
+            // the largest of the row's remaining values, of equal ones the lowest action, `top` times
+            if (known.bad) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) key[i] = x[i] > NONE && !known.bad ? order_key(x[i], (unsigned)short_action<G, E, WIDE>(lane, i)) : 0ull;
-#pragma unroll
-            for (int size = 2; size <= E; size *= 2)
-#pragma unroll
-                for (int by = size / 2; by; by /= 2)
-#pragma unroll
-                    for (int i = 0; i < E; ++i)
-                        if ((i & by) == 0) {
-                            const bool falling = (i & size) == 0 || size == E;
-                            const unsigned long long u = key[i], v = key[i | by];
-                            const bool swap = falling ? u < v : u > v;
-                            key[i] = swap ? v : u; key[i | by] = swap ? u : v;
-                        }
+                for (int i = 0; i < E; ++i) x[i] = NONE;
+            }
             for (int k = 0; k < o.top; ++k) {
-                unsigned long long best = key[0];
+                float high = x[0];
 #pragma unroll
-                for (int by = 1; by < G; by *= 2) { const unsigned long long other = __shfl_xor_sync(ALL, best, by); best = best > other ? best : other; }
-                if (best == 0ull ? lane == 0 : key[0] == best) {
-                    if (write) write_top(o, p, known, r, k, best);
+                for (int i = 1; i < E; ++i) high = fmaxf(high, x[i]);
 #pragma unroll
-                    for (int i = 0; i + 1 < E; ++i) key[i] = key[i + 1];
-                    key[E - 1] = 0ull;
+                for (int by = 1; by < G; by *= 2) high = fmaxf(high, __shfl_xor_sync(ALL, high, by));
+                int at = 0x7FFFFFFF;
+#pragma unroll
+                for (int i = E - 1; i >= 0; --i) at = x[i] == high ? short_action<G, E, WIDE>(lane, i) : at;
+#pragma unroll
+                for (int by = 1; by < G; by *= 2) at = min(at, __shfl_xor_sync(ALL, at, by));
+                const bool there = high > NONE;
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[i] = there && short_action<G, E, WIDE>(lane, i) == at ? NONE : x[i];
+                if (write && lane == 0) {
+                    o.top_actions[r * o.top + k] = there ? at : -1;
+                    o.top_logprobs[r * o.top + k] = known.bad ? known.log2_s : there ? known.logprob(high, p) : NONE;
                 }
             }
         }
@@ -343,20 +354,37 @@ __device__ __forceinline__ float warp_ranked(float v, int rank, unsigned lane) {
     }
     return high;
 }
-// A whole row by the threads of a team the slow way, with exact differences: lane- and warp-wise parts of it (see below for where it is needed).
+// A whole row by the threads of a team a second time, with exact differences: lane- and warp-wise parts of it (see below for where it is needed).
+template <int TYPE, class F> __device__ __forceinline__ void each_chunk(const Row<TYPE>& row, int t, int threads, F f) {
+    constexpr int N = Chunk<TYPE>::N;
+#pragma unroll 4
+    for (int k = t; k < row.chunks; k += threads) {
+        float x[N];
+        Chunk<TYPE>::values(row.chunk(k), x);
+        if (row.legal) {
+            unsigned legal[N / 4];
+            mask_words<N>(row.legal, row.head + k * N, row.actions, legal);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = is_legal<N>(legal, i) ? x[i] : NONE;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(x[i]);
+    }
+    if (t < row.ends) f(row.at(row.end(t)));
+}
 template <int TYPE> __device__ __forceinline__ float exact_max(const Row<TYPE>& row, int t, int threads) {
     float m = NONE;
-    for (int j = t; j < row.actions; j += threads) m = fmaxf(m, row.at(j));
+    each_chunk(row, t, threads, [&](float x) { m = fmaxf(m, x); });
     return warp_max(m);
 }
 template <int TYPE> __device__ __forceinline__ Part exact_sums(const Row<TYPE>& row, float m, float scale, int t, int threads) {
     const float from = m == NONE ? 0.0f : m;
     Part p{m, 0.0f, 0.0f};
-    for (int j = t; j < row.actions; j += threads) {
-        const float y = (row.at(j) - from) * scale * LOG2E, e = exp2_fast(y);
+    each_chunk(row, t, threads, [&](float x) {
+        const float y = (x - from) * scale * LOG2E, e = exp2_fast(y);
         p.s += e;
         p.t += e > 0.0f ? y * e : 0.0f;
-    }
+    });
 #pragma unroll
     for (int by = 16; by; by /= 2) { p.s += __shfl_xor_sync(ALL, p.s, by); p.t += __shfl_xor_sync(ALL, p.t, by); }
     return p;
@@ -378,9 +406,24 @@ __device__ __forceinline__ int place_of(unsigned long long key, const unsigned l
     return place;
 }
 
-template <int TYPE> __device__ __forceinline__ void largest(const float (&x)[Chunk<TYPE>::N], float& m) {
+// A chunk's values with the masked ones at minus infinity, their maximum, then all of them at FLOOR at least.  (bf16 without a mask goes there two values at a time,
+// before the maximum: it is FLOOR then where there is nothing.)
+template <int TYPE, bool MASKED>
+__device__ __forceinline__ void take_chunk(const uint4& raw, const unsigned (&legal)[Chunk<TYPE>::N / 4], float (&x)[Chunk<TYPE>::N], float& m) {
+    constexpr int N = Chunk<TYPE>::N;
+    constexpr bool EARLY = TYPE == CUDARL_BF16 && !MASKED;
+    if constexpr (EARLY) Chunk<TYPE>::floored(raw, x);
+    else Chunk<TYPE>::values(raw, x);
+    if constexpr (MASKED) {
 #pragma unroll
-    for (int i = 0; i < Chunk<TYPE>::N; i += 2) m = max3(m, x[i], x[i + 1]);
+        for (int i = 0; i < N; ++i) x[i] = is_legal<N>(legal, i) ? x[i] : NONE;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 2) m = max3(m, x[i], x[i + 1]);
+    if constexpr (!EARLY) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = max_nan(x[i], FLOOR);
+    }
 }
 template <int TYPE> __device__ __forceinline__ void add_chunk(const float (&x)[Chunk<TYPE>::N], Two c2, Two mc2, Two& s2, Two& t2) {
 #pragma unroll
@@ -393,119 +436,125 @@ template <int TYPE> __device__ __forceinline__ void add_chunk(const float (&x)[C
         t2 = fma2(y2, e2, t2);
     }
 }
-__device__ __forceinline__ float sum2(Two v) { float a, b; apart(v, a, b); return a + b; }
 
 // ------------------------------------------------------------------------------------------------------------------ rows of a warp
-// A warp a row, the whole row in registers: CHUNKS pieces of 16 bytes a lane, and an end.  The alternatives: the `top`-th largest of the lanes' maxima is a bound
-// that `top` values reach; the lanes list what reaches it, and each of those counts how many are larger.
-constexpr int WARP_KEYS = 64;
-
+// A warp a row, the whole row in registers: CHUNKS pieces of 16 bytes a lane, and an end.  What is
+// scalar in a row -- the taken action's logit, logarithm, quotient, addresses, the writes -- is done for up to 32 consecutive rows at a time, a lane each.
+// The alternatives: the `top`-th largest of the lanes' maxima is a bound that `top` values reach; what reaches it is listed, and each of those counts how many
+// are larger.
+constexpr int WARP_KEYS = 64, GROUP_KEYS = 128;
 // Blocks on an SM for which the registers suffice.
 constexpr int warp_blocks(int values) { return values <= 8 ? 5 : values <= 16 ? 4 : 3; }
 
 template <int TYPE, int CHUNKS, bool MASKED, bool TOP>
-__global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_warp(Rows p, Outputs o) {
+__global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_warp(Rows p, Outputs o, int group, bool alike) {
     using C = Chunk<TYPE>;
     constexpr int N = C::N;
-    __shared__ unsigned long long keys_all[TOP ? 8 * WARP_KEYS : 1];
+    __shared__ unsigned long long keys_all[TOP ? 8 * WARP_KEYS : 1], sorted_all[TOP ? 8 * GROUP_KEYS : 1];
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
     unsigned long long* const keys = keys_all + (TOP ? warp * WARP_KEYS : 0u);
+    unsigned long long* const sorted = sorted_all + (TOP ? warp * GROUP_KEYS : 0u);                 // group * top <= GROUP_KEYS
     const float c = p.scale * LOG2E;
-    const long long step = (long long)gridDim.x * 8;
-    uint4 raw[CHUNKS];
-    unsigned legal[CHUNKS][N / 4];
-    float xe_loaded = NONE;
-    int a_loaded = -1;
-    auto load = [&](const Row<TYPE>& row, long long r) {
-        a_loaded = p.taken ? __ldg(p.taken + r) : -1;
-#pragma unroll
-        for (int u = 0; u < CHUNKS; ++u) {
-            const int k = (int)lane + 32 * u;
-            raw[u] = k < row.chunks ? row.chunk(k) : C::fill();
-            if constexpr (MASKED) {
-#pragma unroll
-                for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
-                if (k < row.chunks) mask_words<N>(row.legal, row.head + k * N, row.actions, legal[u]);
+    const long long step = (long long)gridDim.x * 8 * group;
+    long long first = ((long long)blockIdx.x * 8 + warp) * group;
+    Row<TYPE> row(p, first < p.rows ? first : 0);
+    for (; first < p.rows; first += step) {
+        const int rows = (int)min((long long)group, p.rows - first);
+        int a = -1;
+        float xa = NONE;
+        if ((int)lane < rows && p.taken) {
+            a = __ldg(p.taken + first + lane);
+            if ((unsigned)a < (unsigned)p.actions) {
+                const long long r = first + lane;
+                xa = p.legal && !__ldg(p.legal + r * p.legal_stride + a) ? NONE : Of<TYPE>::get(static_cast<const typename Of<TYPE>::T*>(p.logits)[r * p.stride + a]);
             }
         }
-        xe_loaded = (int)lane < row.ends ? row.at(row.end((int)lane)) : NONE;
-    };
-    long long r = (long long)blockIdx.x * 8 + warp;
-    if (r < p.rows) load(Row<TYPE>(p, r), r);
-    for (; r < p.rows; r += step) {
-        const Row<TYPE> row(p, r);
-        const int a = a_loaded;
-        const float xe = max_nan(xe_loaded, FLOOR);
-        const bool taken = (unsigned)a < (unsigned)row.actions;
-        const float xa = taken && lane == 0u ? row.at(a) : NONE;
-        float x[CHUNKS][N], m = fmaxf(xe, FLOOR);
+        Part mine{NONE, 0.0f, 0.0f};                                         // of the lane's row
+        for (int i_row = 0; i_row < rows; ++i_row) {
+            if (alike) row.move_to(p, first + i_row); else row = Row<TYPE>(p, first + i_row);
+            uint4 raw[CHUNKS];
+            unsigned legal[CHUNKS][N / 4];
 #pragma unroll
-        for (int u = 0; u < CHUNKS; ++u) {
-            C::floored(raw[u], x[u]);
-            if constexpr (MASKED) {
+            for (int u = 0; u < CHUNKS; ++u) {
+                const int k = (int)lane + 32 * u;
+                raw[u] = k < row.chunks ? row.chunk(k) : C::fill();
+                if constexpr (MASKED) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[u][i] = is_legal<N>(legal[u], i) ? x[u][i] : FLOOR;
+                    for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
+                    if (k < row.chunks) mask_words<N>(row.legal, row.head + k * N, row.actions, legal[u]);
+                }
             }
-            largest<TYPE>(x[u], m);
-        }
-        if (r + step < p.rows) load(Row<TYPE>(p, r + step), r + step);       // the next row's, on their way while this one is computed
-        const float own = m;
-        m = warp_max(m);
-        Part part{m, 0.0f, 0.0f};
-        if (is_usual(m, c)) {
-            const float mc = base_of(m, c), ye = fmaf(xe, c, -mc), ee = exp2_fast(ye);
-            const Two c2 = two(c, c), mc2 = two(-mc, -mc);
-            Two s2 = two(ee, 0.0f), t2 = two(ye * ee, 0.0f);
+            const float xe = (int)lane < row.ends ? row.at(row.end((int)lane)) : NONE;
+            float x[CHUNKS][N], high[CHUNKS], m = fmaxf(xe, NONE);
 #pragma unroll
-            for (int u = 0; u < CHUNKS; ++u) add_chunk<TYPE>(x[u], c2, mc2, s2, t2);
-            part.s = sum2(s2); part.t = sum2(t2);
+            for (int u = 0; u < CHUNKS; ++u) {
+                high[u] = NONE;
+                take_chunk<TYPE, MASKED>(raw[u], legal[u], x[u], high[u]);
+                m = fmaxf(m, high[u]);
+            }
+            const float own = m;
+            m = warp_max(m);
+            Part part{m, 0.0f, 0.0f};
+            if (is_usual(m, c) || m == NONE) {
+                const float mc = base_of(m, c), ye = fmaf(max_nan(xe, FLOOR), c, -mc), ee = exp2_fast(ye);
+                const Two c2 = two(c, c), mc2 = two(-mc, -mc);
+                Two s2 = two(ee, 0.0f), t2 = two(ye * ee, 0.0f);
 #pragma unroll
-            for (int by = 16; by; by /= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
-        } else {                                                             // beyond the limit
-            m = exact_max(row, (int)lane, 32);
-            part = exact_sums(row, m, p.scale, (int)lane, 32);
-        }
-        const Known known(part);
-        if (lane == 0u) {
-            known.write(o, r);
-            if (o.logprob) o.logprob[r] = known.bad ? known.log2_s : taken ? known.logprob(xa, p) : 0.0f;
-        }
-        if constexpr (TOP) {
-            const float bound = warp_ranked(own, o.top, lane);
-            int n = 0;
-            if (bound > ABOVE_FLOOR && !known.bad) {
-                unsigned mine = 0u;                                          // (values cannot be had from registers by number: they are read again)
-                if (own >= bound) {
+                for (int u = 0; u < CHUNKS; ++u) add_chunk<TYPE>(x[u], c2, mc2, s2, t2);
+                part.s = sum2(s2); part.t = sum2(t2);
+#pragma unroll
+                for (int by = 16; by; by /= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
+            } else {                                                         // beyond the limit
+                m = exact_max(row, (int)lane, 32);
+                part = exact_sums(row, m, p.scale, (int)lane, 32);
+            }
+            if ((int)lane == i_row) mine = part;
+            if constexpr (TOP) {
+                const bool bad = !(part.s == part.s);
+                const float bound = warp_ranked(own, o.top, lane);
+                int n = 0;
+                if (bound > ABOVE_FLOOR && !bad) {
+                    auto list = [&](float v, int j) {
+                        const unsigned who = __ballot_sync(ALL, v >= bound);
+                        if (!who) return;
+                        const int place = n + __popc(who & ((1u << lane) - 1u));
+                        if (v >= bound && place < WARP_KEYS) keys[place] = order_key(v, (unsigned)j);
+                        n += __popc(who);
+                    };
 #pragma unroll
                     for (int u = 0; u < CHUNKS; ++u)
+                        if (__any_sync(ALL, high[u] >= bound)) {
 #pragma unroll
-                        for (int i = 0; i < N; ++i) mine |= x[u][i] >= bound ? 1u << (u * N + i) : 0u;
+                            for (int i = 0; i < N; ++i) list(x[u][i], row.head + ((int)lane + 32 * u) * N + i);
+                        }
+                    list(xe, row.end((int)lane));
+                    __syncwarp();
                 }
-                bool end = xe >= bound;
-                while (true) {
-                    const bool has = mine != 0u || end;
-                    const unsigned who = __ballot_sync(ALL, has);
-                    if (!who) break;
-                    if (has) {
-                        int j;
-                        if (mine) { const int e = __ffs((int)mine) - 1; mine &= mine - 1u; j = row.head + ((int)lane + 32 * (e / N)) * N + e % N; }
-                        else { end = false; j = row.end((int)lane); }
-                        const int place = n + __popc(who & ((1u << lane) - 1u));
-                        if (place < WARP_KEYS) keys[place] = order_key(row.at(j), (unsigned)j);
+                if (n >= o.top && n <= WARP_KEYS) {
+                    for (int l = (int)lane; l < n; l += 32) {
+                        const unsigned long long key = keys[l];
+                        const int place = place_of(key, keys, n);
+                        if (place < o.top) sorted[i_row * o.top + place] = key;
                     }
-                    n += __popc(who);
+                } else {
+                    const unsigned long long best = bad || part.s == 0.0f ? 0ull : best_of_all(row, 0, 32, lane, o.top);
+                    if ((int)lane < o.top) sorted[i_row * o.top + (int)lane] = best;
                 }
                 __syncwarp();
             }
-            if (n >= o.top && n <= WARP_KEYS) {
-                for (int l = (int)lane; l < n; l += 32) {
-                    const unsigned long long key = keys[l];
-                    const int place = place_of(key, keys, n);
-                    if (place < o.top) write_top(o, p, known, r, place, key);
-                }
-            } else {
-                const unsigned long long best = known.bad || known.nothing ? 0ull : best_of_all(row, 0, 32, lane, o.top);
-                if ((int)lane < o.top) write_top(o, p, known, r, (int)lane, best);
+        }
+        const Known known(mine);
+        if ((int)lane < rows) {
+            known.write(o, first + lane);
+            if (o.logprob) o.logprob[first + lane] = known.bad ? known.log2_s : (unsigned)a < (unsigned)p.actions ? known.logprob(xa, p) : 0.0f;
+        }
+        if constexpr (TOP) {
+            for (int l0 = 0; l0 < rows * o.top; l0 += 32) {
+                const int l = l0 + (int)lane, of = min(l / o.top, 31);
+                Known its = known;                                           // of the row that the place belongs to
+                its.m = __shfl_sync(ALL, known.m, of); its.log2_s = __shfl_sync(ALL, known.log2_s, of);
+                its.nothing = __shfl_sync(ALL, known.nothing, of); its.bad = __shfl_sync(ALL, known.bad, of);
+                if (l < rows * o.top) write_top(o, p, its, first, l, sorted[l]);
             }
             __syncwarp();
         }
@@ -520,7 +569,7 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
 // warp, are values of the row, so the `top`-th largest of them is a bound that `top` values reach.  Only batches that reach it are read again -- a few dozen --
 // and of what reaches the bound there each counts how many are larger.  Where too much does (rows of equal values) or too little (fewer than `top` values above
 // FLOOR), every value of the row is gone through again, each warp with its 32 best in registers.
-constexpr int UNROLL = 4, RESIDENT = 1024, TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
+constexpr int UNROLL = 4,  TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
 
 template <int T> struct Shared {
     Part part[T / 32];
@@ -547,10 +596,11 @@ __device__ __forceinline__ int place_in_warp(float v, unsigned lane) {
 }
 
 template <int TYPE, int T, bool MASKED, bool TOP>
-__global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int blocks, int group) {
+__global__ void __launch_bounds__(T, (T == 128 && !MASKED ? 768 : 1024) / T) k_long(Rows p, Outputs o, int blocks, int group) {
     using C = Chunk<TYPE>;
     using Value = typename Of<TYPE>::T;
     constexpr int N = C::N, WARPS = T / 32, BATCH = UNROLL * T;
+    constexpr bool AHEAD = T == 128 && !MASKED;                             // (with a mask the registers do not suffice)
     static_assert(WARPS * 32 <= CANDIDATES, "the warps' best have to fit");
     extern __shared__ __align__(128) unsigned char shared_bytes[];
     __shared__ Shared<T> sh;
@@ -566,38 +616,35 @@ __global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int
         const int batches = (row.chunks + BATCH * blocks - 1) / (BATCH * blocks);      // of this block: the row's batch b * blocks + rank
         const int a = t == 0 && rank == 0 && p.taken ? __ldg(p.taken + r) : -1;
         const bool has_end = rank == 0 && t < row.ends;                      // (ends < 2 N <= 16 <= T)
-        const float xe = has_end ? max_nan(row.at(row.end(t)), FLOOR) : FLOOR;
-        Part part{FLOOR, 0.0f, 0.0f};
+        const float xe = has_end ? row.at(row.end(t)) : NONE;
+        Part part{NONE, 0.0f, 0.0f};
         Two s2 = two(0.0f, 0.0f), t2 = s2;
-        float high = FLOOR;                                                  // of the group of batches
-        for (int b = 0; b < batches; ++b) {
+        float high = NONE;                                                   // of the group of batches
+        uint4 raw[UNROLL];
+        unsigned legal[UNROLL][N / 4];
+        auto load = [&](int b) {
             const int at = (b * blocks + rank) * BATCH + t;
-            uint4 raw[UNROLL];
-            unsigned legal[UNROLL][N / 4];
-            if constexpr (MASKED) {
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) {
-                    const int k = at + u * T;
+            for (int u = 0; u < UNROLL; ++u) {
+                const int k = at + u * T;
+                raw[u] = k < row.chunks ? row.chunk(k) : C::fill();
+                if constexpr (MASKED) {
 #pragma unroll
                     for (int i = 0; i < N / 4; ++i) legal[u][i] = 0u;
                     if (k < row.chunks) mask_words<N>(row.legal, row.head + k * N, row.actions, legal[u]);
                 }
             }
+        };
+        if (AHEAD) load(0);
+        for (int b = 0; b < batches; ++b) {
+            if (!AHEAD) load(b);
+            float x[UNROLL][N], bm = NONE;
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) raw[u] = at + u * T < row.chunks ? row.chunk(at + u * T) : C::fill();
-            float x[UNROLL][N], bm = FLOOR;
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                C::floored(raw[u], x[u]);
-                if constexpr (MASKED) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[u][i] = is_legal<N>(legal[u], i) ? x[u][i] : FLOOR;
-                }
-                largest<TYPE>(x[u], bm);
-            }
+            for (int u = 0; u < UNROLL; ++u) take_chunk<TYPE, MASKED>(raw[u], legal[u], x[u], bm);
+            if (AHEAD && b + 1 < batches) load(b + 1);
             if constexpr (TOP) {
                 high = fmaxf(high, bm);
-                if ((b + 1) % group == 0 || b + 1 == batches) { table[(b / group) * T + t] = Of<TYPE>::put(high); high = FLOOR; }
+                if ((b + 1) % group == 0 || b + 1 == batches) { table[(b / group) * T + t] = Of<TYPE>::put(high); high = NONE; }
             }
             if (bm > part.m) {
                 part.s += sum2(s2); part.t += sum2(t2);
@@ -610,7 +657,7 @@ __global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int
         }
         part.s += sum2(s2); part.t += sum2(t2);
         if (has_end) take_one(part, xe, c);
-        if constexpr (TOP) table[TABLE_ROWS * T + t] = Of<TYPE>::put(xe == xe ? xe : FLOOR);
+        if constexpr (TOP) table[TABLE_ROWS * T + t] = Of<TYPE>::put(xe == xe ? xe : NONE);
         const float own = part.m;                                            // this thread's maximum
 
         join_lanes(part, c);
@@ -630,7 +677,7 @@ __global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int
         team_sync<T>();
         float bound = FLOOR;
         if constexpr (TOP) bound = WARPS > 1 ? sh.high[lane] : own;          // 32 values of the row, one a lane
-        if constexpr (T > 32) part = lane < WARPS ? sh.part[lane] : Part{FLOOR, 0.0f, 0.0f};
+        if constexpr (T > 32) part = lane < WARPS ? sh.part[lane] : Part{NONE, 0.0f, 0.0f};
         if (T > 32 && blocks > 1) {
             if (warp == 0) {
                 if constexpr (TOP) sh.block_high[place_in_warp(bound, lane)] = bound;
@@ -639,12 +686,12 @@ __global__ void __launch_bounds__(T, RESIDENT / T) k_long(Rows p, Outputs o, int
             }
             cluster.sync();
             const Shared<T>* const other = cluster.map_shared_rank(&sh, (int)(lane % (unsigned)blocks));
-            part = (int)lane < blocks ? other->block : Part{FLOOR, 0.0f, 0.0f};
+            part = (int)lane < blocks ? other->block : Part{NONE, 0.0f, 0.0f};
             if constexpr (TOP) bound = other->block_high[lane / (unsigned)blocks];
         }
         if constexpr (TOP) bound = warp_min(place_in_warp(bound, lane) < o.top ? bound : INFINITY);
         float m = warp_max(part.m);
-        if (is_usual(m, c)) {
+        if (is_usual(m, c) || m == NONE) {
             if constexpr (T > 32) join_lanes(part, c, blocks > 1 ? 8 : WARPS);
         } else {                                                             // beyond the limit; every block of a cluster goes through the whole row
             m = exact_max(row, t, T);
@@ -781,28 +828,36 @@ __global__ void __launch_bounds__(256) k_short_backward(Rows p, const float* gra
         const int a = p.taken ? __ldg(p.taken + r) : -1;
         const bool taken = (unsigned)a < (unsigned)p.actions;
         const float gl = taken && grad_logprob ? __ldg(grad_logprob + r) : 0.0f, gh = grad_entropy ? __ldg(grad_entropy + r) : 0.0f;
-        const Part part = sum_short<G, E>(x, p.scale, y, e);
+        bool exact;
+        const Part part = sum_short<G, E>(x, p.scale, y, e, exact);
         const Known known(part);
-        const float A = p.scale * (gl + gh * known.h), B = p.scale * gh * LN2, share = 1.0f / part.s;
-        float ya = FLOOR, ga = 0.0f;
-        int ia = -1;
+        const float A = -p.scale * (gl + gh * known.h), B = -p.scale * gh * LN2, share = __fdividef(1.0f, part.s);
+        // the taken action: 1 - p is the others' share
+        float others = 0.0f, ya = 0.0f, ea = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const int j = short_action<G, E, WIDE>(lane, i);
-            if (taken && j == a) { ya = y[i]; ia = i; }
-            x[i] = x[i] == NONE || known.nothing ? 0.0f : -(e[i] * share) * fmaf(B, y[i] - known.log2_s, A);
+            const bool is = short_action<G, E, WIDE>(lane, i) == a;
+            others += is ? 0.0f : e[i];
+            ya = is ? y[i] : ya; ea = is ? e[i] : ea;
+        }
+#pragma unroll
+        for (int by = 1; by < G; by *= 2) others += __shfl_xor_sync(ALL, others, by);
+        const float ga = fmaf(p.scale * gl, others * share, fmaf(ea * share, B * (ya - known.log2_s), -p.scale * gh * known.h * ea * share));
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            const Two lp2 = add2(two(y[i], y[i + 1]), two(-known.log2_s, -known.log2_s)), p2 = mul2(two(e[i], e[i + 1]), two(share, share));
+            apart(mul2(p2, fma2(two(B, B), lp2, two(A, A))), y[i], y[i + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = taken && short_action<G, E, WIDE>(lane, i) == a ? ga : y[i];
+            if (known.nothing) x[i] = 0.0f;
             if (known.bad) x[i] = known.log2_s;
         }
-        if (ia >= 0) {
-            const float lp = (ya - known.log2_s) * LN2;
-            ga = p.scale * (-gl * expm1f(lp) - gh * exp2_fast(ya) * share * (lp + known.h));
-        }
-        const unsigned char* legal = p.legal ? p.legal + r * p.legal_stride : nullptr;
+        if (p.legal) {
+            const unsigned char* legal = p.legal + r * p.legal_stride;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int j = short_action<G, E, WIDE>(lane, i);
-            if (i == ia && !known.nothing && !known.bad) x[i] = ga;
-            if (legal && j < p.actions && !__ldg(legal + j)) x[i] = 0.0f;
+            for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions && !__ldg(legal + j)) x[i] = 0.0f; }
         }
         if (mine >= p.rows) continue;                                        // (a whole team: nothing of it is waited for)
         auto* at = static_cast<typename O::T*>(grad) + r * grad_stride;
@@ -829,15 +884,26 @@ __global__ void __launch_bounds__(256) k_short_backward(Rows p, const float* gra
 template <int TYPE>
 __device__ __forceinline__ void slope_chunk(const Slope& slope, bool usual, const uint4& raw, int j0, float (&v)[Chunk<TYPE>::N]) {
     constexpr int N = Chunk<TYPE>::N;
-    if (usual && (unsigned)(slope.taken - j0) >= (unsigned)N) {
+    if (usual) {
         const Two c2 = two(slope.c, slope.c), mc2 = two(-slope.mc, -slope.mc), l2 = two(-slope.log2_s, -slope.log2_s), A2 = two(-slope.A, -slope.A), B2 = two(-slope.B, -slope.B);
         Chunk<TYPE>::floored(raw, v);
+        const bool has = (unsigned)(slope.taken - j0) < (unsigned)N;
+        float own = v[0];
+        if (has) {
+#pragma unroll
+            for (int i = 1; i < N; ++i) own = slope.taken - j0 == i ? v[i] : own;
+            own = slope.one(own, slope.taken);
+        }
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const Two lp2 = add2(fma2(two(v[i], v[i + 1]), c2, mc2), l2);
             float a, b;
             apart(lp2, a, b);
             apart(mul2(two(exp2_fast(a), exp2_fast(b)), fma2(B2, lp2, A2)), v[i], v[i + 1]);
+        }
+        if (has) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = slope.taken - j0 == i ? own : v[i];
         }
     } else {
         Chunk<TYPE>::values(raw, v);
@@ -853,7 +919,7 @@ __device__ __forceinline__ void slope_chunk(const Slope& slope, bool usual, cons
     }
 }
 
-// A warp a row, all its chunks at once, the next row's on their way meanwhile.
+// A warp a row, all its chunks at once.
 template <int TYPE, int CHUNKS, bool MASKED>
 __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_warp_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad,
                                                                                               long long grad_stride) {
@@ -862,54 +928,42 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
     constexpr int N = C::N;
     const int lane = (int)threadIdx.x % 32;
     const long long step = (long long)gridDim.x * 8;
-    uint4 raw[CHUNKS];
-    typename O::T end;
-    struct Place { const typename O::T* x; typename O::T* g; const unsigned char* legal; int head, chunks, ends; };
-    auto place = [&](long long r) {
-        Place w;
-        w.x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
-        w.g = static_cast<typename O::T*>(grad) + r * grad_stride;
-        w.legal = MASKED ? p.legal + r * p.legal_stride : nullptr;
-        w.head = min((int)((16u - ((unsigned)reinterpret_cast<uintptr_t>(w.g) & 15u)) & 15u) / (int)sizeof(typename O::T), p.actions);
-        w.chunks = (p.actions - w.head) / N;
-        w.ends = p.actions - w.chunks * N;
-        return w;
-    };
-    auto load = [&](const Place& w) {
-        const bool together = (((unsigned)reinterpret_cast<uintptr_t>(w.x) ^ (unsigned)reinterpret_cast<uintptr_t>(w.g)) & 15u) == 0u;
+    for (long long r = (long long)blockIdx.x * 8 + (int)threadIdx.x / 32; r < p.rows; r += step) {
+        const auto* x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
+        auto* g = static_cast<typename O::T*>(grad) + r * grad_stride;
+        const unsigned char* legal = MASKED ? p.legal + r * p.legal_stride : nullptr;
+        const int head = min((int)((16u - ((unsigned)reinterpret_cast<uintptr_t>(g) & 15u)) & 15u) / (int)sizeof(typename O::T), p.actions);
+        const int chunks = (p.actions - head) / N, ends = p.actions - chunks * N;
+        const bool together = (((unsigned)reinterpret_cast<uintptr_t>(x) ^ (unsigned)reinterpret_cast<uintptr_t>(g)) & 15u) == 0u;
+        uint4 raw[CHUNKS];
+        unsigned mask[CHUNKS][N / 4];
 #pragma unroll
         for (int u = 0; u < CHUNKS; ++u) {
             const int k = lane + 32 * u;
             raw[u] = C::fill();
-            if (k < w.chunks) raw[u] = together ? *reinterpret_cast<const uint4*>(w.x + w.head + k * N) : gather_chunk(w.x + w.head + k * N);
+            if (k < chunks) {
+                raw[u] = together ? *reinterpret_cast<const uint4*>(x + head + k * N) : gather_chunk(x + head + k * N);
+                if constexpr (MASKED) mask_words<N>(legal, head + k * N, p.actions, mask[u]);
+            }
         }
-        if (lane < w.ends) end = w.x[lane < w.head ? lane : w.chunks * N + lane];
-    };
-    long long r = (long long)blockIdx.x * 8 + (int)threadIdx.x / 32;
-    if (r < p.rows) load(place(r));
-    for (; r < p.rows; r += step) {
-        const Place w = place(r);
         const Slope slope(p, stats, grad_logprob, grad_entropy, r);
         const bool usual = slope.usual();
-        float v[CHUNKS][N];
-#pragma unroll
-        for (int u = 0; u < CHUNKS; ++u) slope_chunk<TYPE>(slope, usual, raw[u], w.head + (lane + 32 * u) * N, v[u]);
-        const int je = lane < w.head ? lane : w.chunks * N + lane;
-        const float ve = lane < w.ends ? slope.one(O::get(end), je) : 0.0f;
-        if (r + step < p.rows) load(place(r + step));                        // (another row: what is written below is not read there)
+        if (lane < ends) {
+            const int j = lane < head ? lane : chunks * N + lane;
+            g[j] = O::put(MASKED && !__ldg(legal + j) ? 0.0f : slope.one(O::get(x[j]), j));
+        }
 #pragma unroll
         for (int u = 0; u < CHUNKS; ++u) {
             const int k = lane + 32 * u;
-            if (k >= w.chunks) continue;
+            if (k >= chunks) continue;
+            float v[N];
+            slope_chunk<TYPE>(slope, usual, raw[u], head + k * N, v);
             if constexpr (MASKED) {
-                unsigned mask[N / 4];
-                mask_words<N>(w.legal, w.head + k * N, p.actions, mask);
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[u][i] = is_legal<N>(mask, i) ? v[u][i] : 0.0f;
+                for (int i = 0; i < N; ++i) v[i] = is_legal<N>(mask[u], i) ? v[i] : 0.0f;
             }
-            *reinterpret_cast<uint4*>(w.g + w.head + k * N) = C::pack(v[u]);
+            *reinterpret_cast<uint4*>(g + head + k * N) = C::pack(v);
         }
-        if (lane < w.ends) w.g[je] = O::put(MASKED && !__ldg(w.legal + je) ? 0.0f : ve);
     }
 }
 
@@ -1018,13 +1072,18 @@ cudaError_t launch_short(const Rows& p, const Args& args, bool wide4, bool wide8
 template <int TYPE, int VALUES>
 cudaError_t launch_warp(const Rows& p, const Outputs& o, int sms, cudaStream_t st) {
     constexpr int CHUNKS = VALUES / 32 / Chunk<TYPE>::N;
-    const unsigned most = (unsigned)(sms * warp_blocks(VALUES / 32)), all = blocks_of(p.rows, 8), grid = all < most ? all : most;
+    const unsigned most = (unsigned)(sms * warp_blocks(VALUES / 32));
+    // as many rows for a warp at a time as leave every warp of the GPU some
+    int group = 1;
+    while (group < 32 && group * 2 * (o.top ? o.top : 1) <= GROUP_KEYS && p.rows >= 16ll * group * most) group *= 2;
+    const bool alike = p.stride * (long long)sizeof(typename Of<TYPE>::T) % 16 == 0;
+    const unsigned all = blocks_of(p.rows, 8 * group), grid = all < most ? all : most;
     if (p.legal) {
-        if (o.top) k_warp<TYPE, CHUNKS, true, true><<<grid, 256, 0, st>>>(p, o);
-        else k_warp<TYPE, CHUNKS, true, false><<<grid, 256, 0, st>>>(p, o);
+        if (o.top) k_warp<TYPE, CHUNKS, true, true><<<grid, 256, 0, st>>>(p, o, group, alike);
+        else k_warp<TYPE, CHUNKS, true, false><<<grid, 256, 0, st>>>(p, o, group, alike);
     } else {
-        if (o.top) k_warp<TYPE, CHUNKS, false, true><<<grid, 256, 0, st>>>(p, o);
-        else k_warp<TYPE, CHUNKS, false, false><<<grid, 256, 0, st>>>(p, o);
+        if (o.top) k_warp<TYPE, CHUNKS, false, true><<<grid, 256, 0, st>>>(p, o, group, alike);
+        else k_warp<TYPE, CHUNKS, false, false><<<grid, 256, 0, st>>>(p, o, group, alike);
     }
     return cudaGetLastError();
 }
@@ -1038,15 +1097,14 @@ cudaError_t launch_warp(const Rows& p, const BackwardArgs& b, int sms, cudaStrea
 }
 
 template <int TYPE, int T, bool MASKED, bool TOP>
-cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, int sms, cudaStream_t st) {
+cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, cudaStream_t st) {
     const long long batch = (long long)UNROLL * T * blocks, chunks = p.actions / Chunk<TYPE>::N;
     const int group = (int)((chunks + batch * TABLE_ROWS) / (batch * TABLE_ROWS));
-    const long long resident = (long long)sms * (RESIDENT / T);
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(T);
     cfg.dynamicSmemBytes = TOP ? (size_t)(TABLE_ROWS + 1) * T * sizeof(typename Of<TYPE>::T) : 0;
     cfg.stream = st;
-    cfg.gridDim = dim3((unsigned)((p.rows > resident ? resident : p.rows) * blocks));
+    cfg.gridDim = dim3((unsigned)((p.rows < (1ll << 26) ? p.rows : (1ll << 26)) * blocks));
     cudaLaunchAttribute attr[1];
     if (blocks > 1) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1056,9 +1114,9 @@ cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, int sms, cu
     return cudaLaunchKernelEx(&cfg, k_long<TYPE, T, MASKED, TOP>, p, o, blocks, group);
 }
 template <int TYPE, int T>
-cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, int sms, cudaStream_t st) {
-    if (p.legal) return o.top ? launch_long<TYPE, T, true, true>(p, o, blocks, sms, st) : launch_long<TYPE, T, true, false>(p, o, blocks, sms, st);
-    return o.top ? launch_long<TYPE, T, false, true>(p, o, blocks, sms, st) : launch_long<TYPE, T, false, false>(p, o, blocks, sms, st);
+cudaError_t launch_long(const Rows& p, const Outputs& o, int blocks, cudaStream_t st) {
+    if (p.legal) return o.top ? launch_long<TYPE, T, true, true>(p, o, blocks, st) : launch_long<TYPE, T, true, false>(p, o, blocks, st);
+    return o.top ? launch_long<TYPE, T, false, true>(p, o, blocks, st) : launch_long<TYPE, T, false, false>(p, o, blocks, st);
 }
 
 template <int TYPE>
@@ -1071,14 +1129,11 @@ cudaError_t launch_rows(const Rows& p, const Outputs& o, int sms, cudaStream_t s
     if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, o, sms, st);
     // a cluster for each row where there are too few rows to occupy the GPU, as long as each block still gets half a batch
     int blocks = 1;
-    while (blocks < 8 && p.rows * blocks * 2 <= sms * 2 && (long long)v >= 256ll * Chunk<TYPE>::N * UNROLL / 2 * blocks * 2) blocks *= 2;
-    if (const char* e = getenv("POLICY_BLOCKS")) blocks = atoi(e);
-    const char* e = getenv("POLICY_T");
-    const int T = e ? atoi(e) : 256;
-    if (T == 32) return launch_long<TYPE, 32>(p, o, 1, sms, st);
-    if (T == 64) return launch_long<TYPE, 64>(p, o, blocks, sms, st);
-    if (T == 128) return launch_long<TYPE, 128>(p, o, blocks, sms, st);
-    return launch_long<TYPE, 256>(p, o, blocks, sms, st);
+    while (blocks < 8 && p.rows * blocks < 2ll * sms && (long long)v >= 256ll * Chunk<TYPE>::N * UNROLL * blocks) blocks *= 2;
+    if (blocks > 1) return launch_long<TYPE, 256>(p, o, blocks, st);
+    // a warp for each row where there are enough of them to occupy the GPU and what is done once a row weighs more than the wait for a batch
+    if (v <= 8192 && p.rows >= 8ll * sms) return launch_long<TYPE, 32>(p, o, 1, st);
+    return launch_long<TYPE, 128>(p, o, 1, st);
 }
 
 template <int TYPE>
