@@ -355,9 +355,9 @@ __device__ __forceinline__ float warp_ranked(float v, int rank, unsigned lane) {
     return high;
 }
 // A whole row by the threads of a team a second time, with exact differences: lane- and warp-wise parts of it (see below for where it is needed).
-template <int TYPE, class F> __device__ __forceinline__ void each_chunk(const Row<TYPE>& row, int t, int threads, F f) {
+template <int AT_ONCE, int TYPE, class F> __device__ __forceinline__ void each_chunk(const Row<TYPE>& row, int t, int threads, F f) {
     constexpr int N = Chunk<TYPE>::N;
-#pragma unroll 4
+#pragma unroll AT_ONCE
     for (int k = t; k < row.chunks; k += threads) {
         float x[N];
         Chunk<TYPE>::values(row.chunk(k), x);
@@ -372,15 +372,15 @@ template <int TYPE, class F> __device__ __forceinline__ void each_chunk(const Ro
     }
     if (t < row.ends) f(row.at(row.end(t)));
 }
-template <int TYPE> __device__ __forceinline__ float exact_max(const Row<TYPE>& row, int t, int threads) {
+template <int AT_ONCE, int TYPE> __device__ __forceinline__ float exact_max(const Row<TYPE>& row, int t, int threads) {
     float m = NONE;
-    each_chunk(row, t, threads, [&](float x) { m = fmaxf(m, x); });
+    each_chunk<AT_ONCE>(row, t, threads, [&](float x) { m = fmaxf(m, x); });
     return warp_max(m);
 }
-template <int TYPE> __device__ __forceinline__ Part exact_sums(const Row<TYPE>& row, float m, float scale, int t, int threads) {
+template <int AT_ONCE, int TYPE> __device__ __forceinline__ Part exact_sums(const Row<TYPE>& row, float m, float scale, int t, int threads) {
     const float from = m == NONE ? 0.0f : m;
     Part p{m, 0.0f, 0.0f};
-    each_chunk(row, t, threads, [&](float x) {
+    each_chunk<AT_ONCE>(row, t, threads, [&](float x) {
         const float y = (x - from) * scale * LOG2E, e = exp2_fast(y);
         p.s += e;
         p.t += e > 0.0f ? y * e : 0.0f;
@@ -505,8 +505,8 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
 #pragma unroll
                 for (int by = 16; by; by /= 2) { part.s += __shfl_xor_sync(ALL, part.s, by); part.t += __shfl_xor_sync(ALL, part.t, by); }
             } else {                                                         // beyond the limit
-                m = exact_max(row, (int)lane, 32);
-                part = exact_sums(row, m, p.scale, (int)lane, 32);
+                m = exact_max<1>(row, (int)lane, 32);
+                part = exact_sums<1>(row, m, p.scale, (int)lane, 32);
             }
             if ((int)lane == i_row) mine = part;
             if constexpr (TOP) {
@@ -694,14 +694,14 @@ __global__ void __launch_bounds__(T, (T == 128 && !MASKED ? 768 : 1024) / T) k_l
         if (is_usual(m, c) || m == NONE) {
             if constexpr (T > 32) join_lanes(part, c, blocks > 1 ? 8 : WARPS);
         } else {                                                             // beyond the limit; every block of a cluster goes through the whole row
-            m = exact_max(row, t, T);
+            m = exact_max<4>(row, t, T);
             if constexpr (T > 32) {
                 team_sync<T>();
                 if (lane == 0u) sh.part[warp].m = m;
                 team_sync<T>();
                 m = warp_max(sh.part[lane % WARPS].m);
             }
-            part = exact_sums(row, m, p.scale, t, T);
+            part = exact_sums<4>(row, m, p.scale, t, T);
             if constexpr (T > 32) {
                 team_sync<T>();
                 if (lane == 0u) sh.part[warp] = part;
