@@ -21,14 +21,13 @@ constexpr int BLOCK = CUDARL_ADAMW_BLOCK;
 constexpr int WARPS = 8, THREADS = 32 * (WARPS + 1);     // eight warps that compute, and one that has their next pieces copied
 constexpr int RESIDENT = 3;                    // blocks of threads on an SM
 
-struct alignas(16) Tensor {
+struct Tensor {
     void* param; const void* grad; float* master; void* moment1; void* moment2; float* scale1; float* scale2;
     long long count;
     float lr_scale, decay;
     unsigned char param_type, grad_type;
     unsigned char wide;                       // every array but the gradient begins at an address that bulk copies can start at and eight values can be stored to at once
     unsigned char wide_grad;                  // the gradient does
-    unsigned reserved;
 };
 struct Piece { unsigned tensor, block, blocks, number; };   // `blocks` blocks (1 .. WARPS) of a tensor from its block `block` on, which is number `number` of all
 
@@ -144,29 +143,26 @@ __device__ __forceinline__ bool last_block(unsigned* done) {
 // A piece's arrays as they lie in memory: what is whole blocks of aligned arrays comes by bulk copies, several pieces ahead of the warps that compute; the last,
 // shorter block of a tensor, and arrays that are not aligned, those warps load themselves.  Without the copies ahead all warps of the GPU load, then compute, at
 // the same time: with moments of 8 bits, whose arithmetic takes as long as their memory traffic, the two times then add up.
-template <int BITS> struct Stage {                                           // BITS = 0: the gradients alone
-    unsigned char g[WARPS * BLOCK * 4];
-    unsigned char w[BITS ? WARPS * BLOCK * 4 : 16];
-    unsigned char m[BITS == 32 ? WARPS * BLOCK * 4 : BITS == 8 ? WARPS * BLOCK : 16], v[BITS == 32 ? WARPS * BLOCK * 4 : BITS == 8 ? WARPS * BLOCK : 16];
+struct alignas(16) View {                                                              // a piece of a tensor, addresses at its first value
+    const void* grad; const void* weights; void* param; float* master; void* moment1; void* moment2; float* scale1; float* scale2;
+    unsigned values, copied, blocks, number;                                 // values of the piece, whole blocks of it that come by copies, blocks, number of the first
+    float lr_scale, decay;
+    int grad_type, weight_type, param_type;
+    bool wide;
+};
+template <int BITS> struct Stage {
+    unsigned char g[WARPS * BLOCK * 4], w[WARPS * BLOCK * 4];
+    unsigned char m[WARPS * BLOCK * (BITS / 8)], v[WARPS * BLOCK * (BITS / 8)];
     float scale1[WARPS], scale2[WARPS];
-    Tensor tensor;
-    Piece piece;
+    View view;
 };
 template <int BITS> struct Ring {
     static constexpr int STAGES = BITS == 32 ? 2 : 3;
     Stage<BITS> stage[STAGES];
     unsigned long long full[STAGES], empty[STAGES];
 };
-static_assert(sizeof(Tensor) % 16 == 0 && sizeof(Piece) % 16 == 0 && sizeof(Ring<8>) % 16 == 0 && sizeof(Stage<8>) % 16 == 0 && sizeof(Stage<32>) % 16 == 0 && sizeof(Stage<0>) % 16 == 0,
-              "bulk copies take multiples of 16 bytes");
+static_assert(sizeof(Stage<8>) % 16 == 0 && sizeof(Stage<32>) % 16 == 0, "bulk copies go to multiples of 16 bytes");
 __device__ __forceinline__ void copy4(void* to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(to)), "l"(from) : "memory"); }
-
-// Of a piece: how many of its blocks come by copies.
-template <int BITS> __device__ __forceinline__ unsigned copied_blocks(const Tensor& t, const Piece& pc) {
-    const long long whole = t.count / BLOCK - pc.block;
-    if (!t.wide_grad || (BITS && !t.wide)) return 0u;
-    return whole < (long long)pc.blocks ? (unsigned)max(whole, 0ll) : pc.blocks;
-}
 
 template <int BITS> __device__ void init_ring(Ring<BITS>& ring) {
     if (threadIdx.x == 0u)
@@ -174,8 +170,8 @@ template <int BITS> __device__ void init_ring(Ring<BITS>& ring) {
     __syncthreads();
 }
 
-// The copying warp.  Its lanes look up 32 pieces at a time, then each has its own copied when its turn and a stage come.
-template <int BITS> __device__ void copy_pieces(Ring<BITS>& ring, const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl) {
+// The copying warp (a call of its own: its registers are not the computing warps').  Its lanes look up 32 pieces at a time, then each has its own copied when its turn and a stage come.
+template <int BITS> __device__ __noinline__ void copy_pieces(Ring<BITS>& ring, const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl) {
     const unsigned lane = threadIdx.x % 32u;
     unsigned at = 0u, parity = 1u;                                           // the stage that is next, and which phase of `empty` lets it be filled
     bool fine = true;
@@ -183,6 +179,19 @@ template <int BITS> __device__ void copy_pieces(Ring<BITS>& ring, const Tensor* 
         const unsigned long long k = base + (unsigned long long)lane * gridDim.x;
         const Piece pc = k < n ? pieces[k] : Piece{0u, 0u, 0u, 0u};
         const Tensor t = k < n ? tensors[pc.tensor] : Tensor{};
+        const long long first = (long long)pc.block * BLOCK;
+        const unsigned of_g = t.grad_type == CUDARL_F32 ? 4u : 2u, of_p = t.param_type == CUDARL_F32 ? 4u : 2u, of_w = t.master ? 4u : of_p, of_m = BITS / 8;
+        auto moved = [&](void* p, unsigned of) { return p ? static_cast<void*>(static_cast<char*>(p) + first * of) : nullptr; };
+        View view;
+        view.grad = moved(const_cast<void*>(t.grad), of_g); view.param = moved(t.param, of_p); view.master = static_cast<float*>(moved(t.master, 4u));
+        view.weights = t.master ? view.master : view.param;
+        view.moment1 = moved(t.moment1, of_m); view.moment2 = moved(t.moment2, of_m);
+        view.scale1 = t.scale1 + pc.block; view.scale2 = t.scale2 + pc.block;
+        view.values = (unsigned)min(t.count - first, (long long)(WARPS * BLOCK)); view.blocks = pc.blocks; view.number = pc.number;
+        view.copied = t.wide && t.wide_grad ? view.values / BLOCK : 0u;
+        view.lr_scale = t.lr_scale; view.decay = t.decay;
+        view.grad_type = t.grad_type; view.param_type = t.param_type; view.weight_type = t.master ? CUDARL_F32 : t.param_type;
+        view.wide = t.wide;
         for (unsigned turn = 0; turn < 32u && base + (unsigned long long)turn * gridDim.x < n && fine; ++turn) {
             Stage<BITS>& st = ring.stage[at];
             unsigned long long* const bar = &ring.full[at];
@@ -190,26 +199,21 @@ template <int BITS> __device__ void copy_pieces(Ring<BITS>& ring, const Tensor* 
             fine = __shfl_sync(~0u, fine, turn);
             if (!fine) break;
             if (BITS == 8) {                                                 // the scales of its blocks lie anywhere: a lane copies each
-                const float* const scale1 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(t.scale1 + pc.block), turn));
-                const float* const scale2 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(t.scale2 + pc.block), turn));
+                const float* const scale1 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(view.scale1), turn));
+                const float* const scale2 = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(view.scale2), turn));
                 const unsigned blocks = __shfl_sync(~0u, pc.blocks, turn), which = lane % WARPS;
                 if (lane < 2u * WARPS && which < blocks) copy4(lane < WARPS ? &st.scale1[which] : &st.scale2[which], (lane < WARPS ? scale1 : scale2) + which);
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
             }
             if (lane == turn) {
-                const unsigned values = copied_blocks<BITS>(t, pc) * BLOCK;
-                const long long first = (long long)pc.block * BLOCK;
-                const unsigned of_g = t.grad_type == CUDARL_F32 ? 4u : 2u, of_w = t.master || t.param_type == CUDARL_F32 ? 4u : 2u, of_m = BITS == 32 ? 4u : 1u;
-                mbar_arrive_expect_tx(bar, (unsigned)(sizeof(Tensor) + sizeof(Piece)) + values * (of_g + (BITS ? of_w + 2u * of_m : 0u)));
-                bulk_g2s(&st.tensor, tensors + pc.tensor, sizeof(Tensor), bar);
-                bulk_g2s(&st.piece, pieces + k, sizeof(Piece), bar);
+                const unsigned values = view.copied * BLOCK;
+                st.view = view;
+                mbar_publish_expect_tx(bar, values * (of_g + of_w + 2u * of_m));
                 if (values) {
-                    bulk_g2s(st.g, static_cast<const char*>(t.grad) + first * of_g, values * of_g, bar);
-                    if (BITS) {
-                        bulk_g2s(st.w, (t.master ? reinterpret_cast<const char*>(t.master) : static_cast<const char*>(t.param)) + first * of_w, values * of_w, bar);
-                        bulk_g2s(st.m, static_cast<const char*>(t.moment1) + first * of_m, values * of_m, bar);
-                        bulk_g2s(st.v, static_cast<const char*>(t.moment2) + first * of_m, values * of_m, bar);
-                    }
+                    bulk_g2s(st.g, view.grad, values * of_g, bar);
+                    bulk_g2s(st.w, view.weights, values * of_w, bar);
+                    bulk_g2s(st.m, view.moment1, values * of_m, bar);
+                    bulk_g2s(st.v, view.moment2, values * of_m, bar);
                 }
             }
             __syncwarp();
@@ -238,52 +242,61 @@ __device__ __forceinline__ void unstage8(Raw& r, const unsigned char* from, int 
     }
 }
 
-// The sum of the computing warps' values in thread 0, always in the same order.
+// The block's sum in thread 0, always in the same order.
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double warp_sum[WARPS];
     for (int by = 16; by; by /= 2) v += __shfl_xor_sync(~0u, v, by);
     __syncthreads();
-    if (threadIdx.x % 32u == 0u && threadIdx.x / 32u < WARPS) warp_sum[threadIdx.x / 32u] = v;
+    if (threadIdx.x % 32u == 0u) warp_sum[threadIdx.x / 32u] = v;
     __syncthreads();
     v = warp_sum[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) v += warp_sum[w];
     return v;
 }
-
-// Sum of squares of all gradients, in 64 bits and in an order that only the list of pieces and the grid make; the last block adds the blocks' sums.
-__global__ void __launch_bounds__(THREADS, RESIDENT) k_grad_norm(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
-    asm volatile("griddepcontrol.launch_dependents;");                       // the step's blocks may come as these go: they load before they wait for the norm
-    extern __shared__ __align__(128) unsigned char shared_bytes[];
-    Ring<0>& ring = *reinterpret_cast<Ring<0>*>(shared_bytes);
-    init_ring(ring);
-    double sum = 0.0;
-    const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
-    if (warp == WARPS) copy_pieces(ring, tensors, pieces, n, ctl);
-    else {
-        unsigned at = 0u, parity = 0u;
-        for (unsigned long long k = blockIdx.x; k < n; k += gridDim.x) {
-            Stage<0>& st = ring.stage[at];
-            if (!mbar_wait(&ring.full[at], parity, 0u)) { if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT); break; }
-            const Piece pc = st.piece;
-            const int type = st.tensor.grad_type;
-            Raw raw;
-            const bool mine = warp < pc.blocks;
-            if (mine) {
-                if (warp < copied_blocks<0>(st.tensor, pc)) unstage8(raw, st.g, type, warp, lane);
-                else {
-                    const long long from = (long long)(pc.block + warp) * BLOCK + lane * 8u;
-                    load8(raw, st.tensor.grad, type, from, false, (int)min(8ll, st.tensor.count - from));
-                }
-            }
-            __syncwarp();
-            if (lane == 0u) mbar_arrive(&ring.empty[at]);
-            if (++at == Ring<0>::STAGES) { at = 0u; parity ^= 1u; }
-            if (!mine) continue;
-            float g[8];
-            floats8(raw, type, g);
+// Squares of eight values of each of COUNT blocks, all loads first.
+template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(double& sum, const void* grad, long long at) {
+    Raw raw[COUNT];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+    for (int u = 0; u < COUNT; ++u) load8(raw[u], grad, TYPE, at + u * BLOCK, true, 8);
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+        float g[8];
+        floats8(raw[u], TYPE, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+    }
+}
+
+// Sum of squares of all gradients, in 64 bits and in an order that only the list of pieces and the grid make; the last block adds the blocks' sums.  A warp a
+// piece, 64 (32 bits) or 128 bytes a lane on their way at a time: as many conversions to 64 bits as take about two thirds of the time that the bytes take.
+__global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tensors, const Piece* __restrict__ pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
+    asm volatile("griddepcontrol.launch_dependents;");                       // the step's blocks may come as these go: they load before they wait for the norm
+    double sum = 0.0;
+    const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, stride = gridDim.x * WARPS;
+    unsigned k = blockIdx.x * WARPS + warp;                                  // (no overflow: at most 2^26 pieces)
+    Piece next = k < n ? pieces[k] : Piece{0u, 0u, 0u, 0u};
+    for (; k < n; k += stride) {
+        const Piece pc = next;
+        if (k + stride < n) next = pieces[k + stride];
+        const Tensor& t = tensors[pc.tensor];
+        const int type = t.grad_type;
+        const void* const grad = t.grad;
+        const long long first = (long long)pc.block * BLOCK, at = first + lane * 8u, left = t.count - first;
+        if (t.wide_grad && left >= WARPS * BLOCK) {
+            static_assert(WARPS == 8, "the blocks of a whole piece");
+            if (type == CUDARL_F32) { add_squares<CUDARL_F32, 4>(sum, grad, at); add_squares<CUDARL_F32, 4>(sum, grad, at + 4 * BLOCK); }
+            else if (type == CUDARL_BF16) add_squares<CUDARL_BF16, 8>(sum, grad, at);
+            else add_squares<CUDARL_F16, 8>(sum, grad, at);
+        } else {
+            for (unsigned u = 0; u < pc.blocks; ++u) {
+                Raw raw;
+                float g[8];
+                load8(raw, grad, type, at + u * BLOCK, false, (int)min(8ll, left - (long long)(u * BLOCK + lane * 8u)));
+                floats8(raw, type, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+            }
         }
     }
     sum = block_sum(sum);
@@ -297,8 +310,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_grad_norm(const Tensor* t
     __syncthreads();
     if (!last) return;
     sum = 0.0;
-    if (threadIdx.x < 32u * WARPS)
-        for (unsigned b = threadIdx.x; b < gridDim.x; b += 32u * WARPS) sum += __ldcg(part + b);
+    for (unsigned b = threadIdx.x; b < gridDim.x; b += 32u * WARPS) sum += __ldcg(part + b);
     sum = block_sum(sum);
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum) * fabs((double)grad_scale);
@@ -353,52 +365,38 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
     const float fix1 = __ldcg(&ctl->fix1), root_fix2 = __ldcg(&ctl->root_fix2);
     const bool go = !s.clipped || __ldcg(&ctl->go);
     const float scale = s.clipped ? grad_scale * __ldcg(&ctl->clip) : grad_scale;
+    unsigned prefix[4];
+    policy_prefix(s.keys, (unsigned long long)(step + 1), prefix);
     unsigned place = 0u, parity = 0u;
     for (unsigned long long k = blockIdx.x; k < n && !copies; k += gridDim.x) {
         Stage<BITS>& st = ring.stage[place];
         unsigned long long* const empty = &ring.empty[place];
         if (!mbar_wait(&ring.full[place], parity, 0u)) { if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT); break; }
         if (++place == Ring<BITS>::STAGES) { place = 0u; parity ^= 1u; }
-        const Piece pc = st.piece;
-        if (warp >= pc.blocks || !go) {
-            __syncwarp();
-            if (lane == 0u) mbar_arrive(empty);
-            continue;
-        }
-        const Tensor t = st.tensor;
-        const unsigned block = pc.block + warp;
-        const long long at = (long long)block * BLOCK + lane * 8u;
-        const int len = (int)min(8ll, t.count - at);                         // of this lane's eight
-        const bool wide = t.wide && len == 8;
-        const int grad_type = t.grad_type, param_type = t.param_type;
-        float* const master = t.master;
-        void* const param = t.param;
-        void* const moment1 = t.moment1;
-        void* const moment2 = t.moment2;
-        float* const at_scale1 = t.scale1 + block;
-        float* const at_scale2 = t.scale2 + block;
-        const float rate = lr * t.lr_scale, decay = t.decay;
-        const int weight_type = master ? CUDARL_F32 : param_type;
+        const View& view = st.view;
+        if (warp < view.blocks && go) {
+        const unsigned at = warp * BLOCK + lane * 8u;
+        const int len = min(8, (int)view.values - (int)at);                  // of this lane's eight
+        const bool wide = view.wide && len == 8;
+        const float rate = lr * view.lr_scale, decay = view.decay;
         Raw gr, wr, mr, vr;
         uint2 c1 = make_uint2(0u, 0u), c2 = c1;
         float old1 = 0.0f, old2 = 0.0f;
-        if (warp < copied_blocks<BITS>(t, pc)) {
-            unstage8(gr, st.g, grad_type, warp, lane);
-            unstage8(wr, st.w, weight_type, warp, lane);
+        if (warp < view.copied) {
+            unstage8(gr, st.g, view.grad_type, warp, lane);
+            unstage8(wr, st.w, view.weight_type, warp, lane);
             if (BITS == 32) { unstage8(mr, st.m, CUDARL_F32, warp, lane); unstage8(vr, st.v, CUDARL_F32, warp, lane); }
             else { c1 = reinterpret_cast<const uint2*>(st.m)[warp * 32u + lane]; c2 = reinterpret_cast<const uint2*>(st.v)[warp * 32u + lane]; }
         } else {
-            load8(gr, t.grad, grad_type, at, false, len);
-            load8(wr, master ? master : param, weight_type, at, false, len);
-            if (BITS == 32) { load8(mr, moment1, CUDARL_F32, at, false, len); load8(vr, moment2, CUDARL_F32, at, false, len); }
-            else { c1 = load_codes(moment1, at, false, len); c2 = load_codes(moment2, at, false, len); }
+            load8(gr, view.grad, view.grad_type, at, false, len);
+            load8(wr, view.weights, view.weight_type, at, false, len);
+            if (BITS == 32) { load8(mr, view.moment1, CUDARL_F32, at, false, len); load8(vr, view.moment2, CUDARL_F32, at, false, len); }
+            else { c1 = load_codes(view.moment1, at, false, len); c2 = load_codes(view.moment2, at, false, len); }
         }
         if (BITS == 8) { old1 = st.scale1[warp]; old2 = st.scale2[warp]; }
-        __syncwarp();
-        if (lane == 0u) mbar_arrive(empty);                                  // the stage can be filled again
         float g[8], w[8], m[8], v[8];
-        floats8(gr, grad_type, g);
-        floats8(wr, weight_type, w);
+        floats8(gr, view.grad_type, g);
+        floats8(wr, view.weight_type, w);
         if (BITS == 32) { floats8(mr, CUDARL_F32, m); floats8(vr, CUDARL_F32, v); }
         if (BITS == 8) {
             from_codes(c1.x, m); from_codes(c1.y, m + 4); from_codes(c2.x, v); from_codes(c2.y, v + 4);
@@ -423,18 +421,18 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
             apart(fma2(negative2(rate), fma2(two(decay, decay), wi, way), wi), w[i], w[i + 1]);
             apart(mi, m[i], m[i + 1]); apart(vi, v[i], v[i + 1]); apart(ri, root[i], root[i + 1]);
         }
-        if (master) store8(master, CUDARL_F32, at, wide, len, w);
-        store8(param, param_type, at, wide, len, w);
+        if (view.master) store8(view.master, CUDARL_F32, at, wide, len, w);
+        store8(view.param, view.param_type, at, wide, len, w);
         if (BITS == 32) {
-            store8(moment1, CUDARL_F32, at, wide, len, m);
-            store8(moment2, CUDARL_F32, at, wide, len, v);
+            store8(view.moment1, CUDARL_F32, at, wide, len, m);
+            store8(view.moment2, CUDARL_F32, at, wide, len, v);
         } else {
             // the largest magnitudes, in the order of their bits (values behind the tensor's end are zeros; NaN is the largest)
             float top1 = 0.0f, top2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) { top1 = max_nan(top1, fabsf(m[i]), fabsf(m[i + 1])); top2 = max_nan(top2, root[i], root[i + 1]); }
             const float scale1 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top1))) * (1.0f / 448.0f), scale2 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top2))) * (1.0f / 448.0f);
-            if (lane == 0) { *at_scale1 = scale1; *at_scale2 = scale2; }
+            if (lane == 0) { view.scale1[warp] = scale1; view.scale2[warp] = scale2; }
             float y1[8], y2[8], least = 448.0f;
             const bool usual = scale1 > 7.9e-31f && scale1 < 1.2e30f && scale2 > 7.9e-31f && scale2 < 1.2e30f;
             if (usual) {
@@ -454,8 +452,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
             unsigned d1[2], d2[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const unsigned long long quad = (unsigned long long)(pc.number + warp) * (BLOCK / 4) + lane * 2u + q;
-                const U4 r = philox4x32_10((unsigned)quad, (unsigned)(quad >> 32), (unsigned)(step + 1), (unsigned)((unsigned long long)(step + 1) >> 32), s.keys);
+                const U4 r = policy_philox((view.number + warp) * (BLOCK / 4u) + lane * 2u + q, s.keys, prefix);      // counter (quad, 0, step): quads stay below 2^32
                 const unsigned word[4] = {r.x, r.y, r.z, r.w};
                 unsigned a[4], b[4];                                         // a code in the top byte of each
                 if (all_normal) {
@@ -476,9 +473,12 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
                 d1[q] = __byte_perm(__byte_perm(a[0], a[1], 0x0073u), __byte_perm(a[2], a[3], 0x0073u), 0x5410u);
                 d2[q] = __byte_perm(__byte_perm(b[0], b[1], 0x0073u), __byte_perm(b[2], b[3], 0x0073u), 0x5410u);
             }
-            store_codes(moment1, at, wide, len, make_uint2(d1[0], d1[1]));
-            store_codes(moment2, at, wide, len, make_uint2(d2[0], d2[1]));
+            store_codes(view.moment1, at, wide, len, make_uint2(d1[0], d1[1]));
+            store_codes(view.moment2, at, wide, len, make_uint2(d2[0], d2[1]));
         }
+        }
+        __syncwarp();
+        if (lane == 0u) mbar_arrive(empty);                                  // the stage can be filled again
     }
     if (last_block(&ctl->done)) {
         if (go) {
@@ -498,13 +498,13 @@ struct cudarl_adamw {
     Piece* dpieces = nullptr;
     Control* dctl = nullptr;
     double* dpart = nullptr;
-    unsigned pieces = 0, grid = 0;
+    unsigned pieces = 0, grid = 0, norm_grid = 0;
     bool gradients = false;                  // every tensor with values has one
 };
 
 namespace {
 
-size_t ring_bytes(int bits) { return bits == 8 ? sizeof(Ring<8>) : bits == 32 ? sizeof(Ring<32>) : sizeof(Ring<0>); }
+size_t ring_bytes(int bits) { return bits == 8 ? sizeof(Ring<8>) : sizeof(Ring<32>); }
 
 int check_tensor(const cudarl_adamw_tensor& t, int bits, CallerArrays& arrays) {
     if (t.count < 0 || t.count > (1ll << 40)) return fail_global(-1, "count of a tensor out of range");
@@ -545,7 +545,7 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
         const cudarl_adamw_tensor& t = tensors[i];
         const int rc = check_tensor(t, o->cfg.state_bits, arrays);
         if (rc) return rc;
-        Tensor d{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.lr_scale, t.weight_decay, (unsigned char)t.param_type, (unsigned char)t.grad_type, 0, 0, 0};
+        Tensor d{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.lr_scale, t.weight_decay, (unsigned char)t.param_type, (unsigned char)t.grad_type, 0, 0};
         auto eight = [](const void* p, size_t value) { return reinterpret_cast<uintptr_t>(p) % (8 * value) == 0; };
         auto sixteen = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
         const size_t moment = o->cfg.state_bits == 8 ? 1 : 4;
@@ -553,7 +553,7 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
         d.wide_grad = sixteen(t.grad);
         o->tensors.push_back(d);
         const int64_t blocks = (t.count + BLOCK - 1) / BLOCK;
-        if (number + blocks > (1ll << 31)) return fail_global(-1, "more than 2^39 values in one handle");
+        if (number + blocks > (1ll << 26)) return fail_global(-1, "more than 2^34 values in one handle");
         for (int64_t b = 0; b < blocks; b += WARPS) pieces.push_back(Piece{(unsigned)i, (unsigned)b, (unsigned)std::min<int64_t>(WARPS, blocks - b), (unsigned)(number + b)});
         number += blocks;
     }
@@ -566,6 +566,8 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, o->cfg.device)) != cudaSuccess) return fail_cuda("cudaDeviceGetAttribute", e);
     const unsigned most = (unsigned)(sms * RESIDENT), blocks = o->pieces;
     o->grid = blocks < 1u ? 1u : blocks < most ? blocks : most;
+    const unsigned norm_most = (unsigned)(sms * 4), norm_blocks = (o->pieces + WARPS - 1) / WARPS;
+    o->norm_grid = norm_blocks < 1u ? 1u : norm_blocks < norm_most ? norm_blocks : norm_most;
     Control c;
     std::memset(&c, 0, sizeof c);
     c.step = o->cfg.step;
@@ -574,7 +576,7 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
     c.fix1 = (float)(1.0 / (1.0 - c.power1)); c.root_fix2 = (float)std::sqrt(1.0 / (1.0 - c.power2));
     c.clip = 1.0f;
     if ((e = cudaMalloc(&o->dtensors, sizeof(Tensor) * (o->tensors.size() + 1))) != cudaSuccess || (e = cudaMalloc(&o->dpieces, sizeof(Piece) * (pieces.size() + 1))) != cudaSuccess ||
-        (e = cudaMalloc(&o->dctl, sizeof(Control))) != cudaSuccess || (e = cudaMalloc(&o->dpart, sizeof(double) * o->grid)) != cudaSuccess) return fail_cuda("cudaMalloc", e);
+        (e = cudaMalloc(&o->dctl, sizeof(Control))) != cudaSuccess || (e = cudaMalloc(&o->dpart, sizeof(double) * o->norm_grid)) != cudaSuccess) return fail_cuda("cudaMalloc", e);
     if ((e = cudaMemcpy(o->dtensors, o->tensors.data(), sizeof(Tensor) * o->tensors.size(), cudaMemcpyHostToDevice)) != cudaSuccess ||
         (e = cudaMemcpy(o->dpieces, pieces.data(), sizeof(Piece) * pieces.size(), cudaMemcpyHostToDevice)) != cudaSuccess ||
         (e = cudaMemcpy(o->dctl, &c, sizeof c, cudaMemcpyHostToDevice)) != cudaSuccess || (e = cudaDeviceSynchronize()) != cudaSuccess) return fail_cuda("cudaMemcpy", e);
@@ -627,7 +629,7 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
         s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;
     }
     if (s.clipped) {
-        k_grad_norm<<<o->grid, THREADS, ring_bytes(0), st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, grad_scale, c.max_grad_norm);
+        k_grad_norm<<<o->norm_grid, 32 * WARPS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, grad_scale, c.max_grad_norm);
         if ((e = cudaGetLastError()) != cudaSuccess) return fail_cuda("cudarl_adamw_step", e);
     }
     cudaLaunchConfig_t launch = {};

@@ -13,6 +13,10 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(unsigned long long* bar, u
     // relaxed: the barrier only tells this warp that its tensor copy has landed; no write of the arriving lane is published by it
     asm volatile("mbarrier.arrive.expect_tx.relaxed.cta.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// The same by a lane that has written to shared memory itself what the barrier's waiters read.
+__device__ __forceinline__ void mbar_publish_expect_tx(unsigned long long* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory"); }
 // One look at the barrier, no waiting.
 __device__ __forceinline__ bool mbar_test_wait(unsigned long long* bar, unsigned parity) {

@@ -314,7 +314,7 @@ typedef struct cudarl_adamw_stats {
 typedef struct cudarl_adamw cudarl_adamw;
 
 /* The handle keeps the list of the tensors and the step count on the device; the tensors' memory stays the caller's and has
- * to outlive it.  Tensors must not overlap.  One handle's calls are ordered by the caller (one stream, or events). */
+ * to outlive it.  At most 2^34 values, in blocks of 256 counted up for every tensor.  Tensors must not overlap.  One handle's calls are ordered by the caller (one stream, or events). */
 int  cudarl_adamw_create(const cudarl_adamw_config* cfg, int32_t count, const cudarl_adamw_tensor* tensors, cudarl_adamw** out);
 /* Waits for the device. */
 void cudarl_adamw_destroy(cudarl_adamw* opt);
