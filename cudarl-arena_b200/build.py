@@ -64,7 +64,7 @@ def build_lib(force=False):
     srcs = [s for s in srcs if os.path.exists(s)]
     if not force and _newer(LIB, deps):
         return LIB
-    cmd = [_nvcc()] + NVCC_FLAGS + ["-shared", "-o", LIB] + srcs + ["-I" + os.path.join(ROOT, "include"), "-ldl", "-lpthread"]
+    cmd = [_nvcc()] + NVCC_FLAGS + ["--threads", "0", "-shared", "-o", LIB] + srcs + ["-I" + os.path.join(ROOT, "include"), "-ldl", "-lpthread"]
     _run(cmd, log=os.path.join(HERE, "build_libcudarl.log"))
     return LIB
 

@@ -255,7 +255,7 @@ __device__ __forceinline__ double block_sum(double v) {
     return v;
 }
 // Squares of eight values of each of COUNT blocks, all loads first.
-template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(double& sum, const void* grad, long long at) {
+template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(double (&sum)[4], const void* grad, long long at) {
     Raw raw[COUNT];
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) load8(raw[u], grad, TYPE, at + u * BLOCK, true, 8);
@@ -264,7 +264,7 @@ template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(doubl
         float g[8];
         floats8(raw[u], TYPE, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+        for (int i = 0; i < 8; ++i) sum[i % 4] = fma((double)g[i], (double)g[i], sum[i % 4]);
     }
 }
 
@@ -272,7 +272,7 @@ template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(doubl
 // piece, 64 (32 bits) or 128 bytes a lane on their way at a time: as many conversions to 64 bits as take about two thirds of the time that the bytes take.
 __global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tensors, const Piece* __restrict__ pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
     asm volatile("griddepcontrol.launch_dependents;");                       // the step's blocks may come as these go: they load before they wait for the norm
-    double sum = 0.0;
+    double four[4] = {0.0, 0.0, 0.0, 0.0};                                   // (four sums in turn: additions of 64 bits take their time)
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, stride = gridDim.x * WARPS;
     unsigned k = blockIdx.x * WARPS + warp;                                  // (no overflow: at most 2^26 pieces)
     Piece next = k < n ? pieces[k] : Piece{0u, 0u, 0u, 0u};
@@ -285,9 +285,9 @@ __global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tenso
         const long long first = (long long)pc.block * BLOCK, at = first + lane * 8u, left = t.count - first;
         if (t.wide_grad && left >= WARPS * BLOCK) {
             static_assert(WARPS == 8, "the blocks of a whole piece");
-            if (type == CUDARL_F32) { add_squares<CUDARL_F32, 4>(sum, grad, at); add_squares<CUDARL_F32, 4>(sum, grad, at + 4 * BLOCK); }
-            else if (type == CUDARL_BF16) add_squares<CUDARL_BF16, 8>(sum, grad, at);
-            else add_squares<CUDARL_F16, 8>(sum, grad, at);
+            if (type == CUDARL_F32) { add_squares<CUDARL_F32, 4>(four, grad, at); add_squares<CUDARL_F32, 4>(four, grad, at + 4 * BLOCK); }
+            else if (type == CUDARL_BF16) add_squares<CUDARL_BF16, 8>(four, grad, at);
+            else add_squares<CUDARL_F16, 8>(four, grad, at);
         } else {
             for (unsigned u = 0; u < pc.blocks; ++u) {
                 Raw raw;
@@ -295,11 +295,11 @@ __global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tenso
                 load8(raw, grad, type, at + u * BLOCK, false, (int)min(8ll, left - (long long)(u * BLOCK + lane * 8u)));
                 floats8(raw, type, g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += (double)g[i] * (double)g[i];
+                for (int i = 0; i < 8; ++i) four[i % 4] = fma((double)g[i], (double)g[i], four[i % 4]);
             }
         }
     }
-    sum = block_sum(sum);
+    double sum = block_sum((four[0] + four[1]) + (four[2] + four[3]));
     __shared__ bool last;
     if (threadIdx.x == 0) {
         part[blockIdx.x] = sum;

@@ -47,6 +47,16 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
     const unsigned b = (unsigned)(key >> 32);
     return __uint_as_float((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b);
 }
+// The same for a value of 16 bits and an action below 2^16, in 32 bits.
+template <int TYPE> __device__ __forceinline__ unsigned order_key16(float x, unsigned action) {
+    x += 0.0f;
+    const unsigned b = TYPE == CUDARL_BF16 ? __float_as_uint(x) >> 16 : (unsigned)__half_as_ushort(__float2half_rn(x));
+    return ((b & 0x8000u) ? ~b & 0xFFFFu : b | 0x8000u) << 16 | (0xFFFFu - action);
+}
+template <int TYPE> __device__ __forceinline__ float key16_value(unsigned key) {
+    const unsigned b = (key & 0x80000000u) ? key >> 16 & 0x7FFFu : ~(key >> 16) & 0xFFFFu;
+    return TYPE == CUDARL_BF16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half((unsigned short)b));
+}
 __device__ __forceinline__ int key_action(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
 
 // A part of a row: its maximum, and the sums with the maximum's m c taken off -- or -LIMIT where that is more: a part so low (a masked one, or an empty one)
@@ -294,43 +304,69 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
         const int a = p.taken ? __ldg(p.taken + r) : -1;
         bool exact;
         const Known known(sum_short<G, E>(x, p.scale, y, e, exact));
-        if (write) {
-            if (lane == 0 && o.entropy) o.entropy[r] = known.h;
+        const bool rare = exact || known.bad;
+        const float c = p.scale * LOG2E, base = -(known.m * c);
+        auto logprob = [&](float v) { return rare || v < -LARGE ? known.logprob(v, p) : LN2 * (fmaf(v, c, base) - known.log2_s); };
+        if (write && lane == 0) {
+            if (o.entropy) o.entropy[r] = known.h;
             if (o.logprob) {
-                float xa = x[0], ya = y[0];
-                bool has = a == short_action<G, E, WIDE>(lane, 0);
+                float lp = known.bad ? known.log2_s : 0.0f;
+                if constexpr (G == 1) {                                      // the lane has it
+                    float xa = x[0];
 #pragma unroll
-                for (int i = 1; i < E; ++i) { const bool is = a == short_action<G, E, WIDE>(lane, i); xa = is ? x[i] : xa; ya = is ? y[i] : ya; has = has || is; }
-                const bool none = (unsigned)a >= (unsigned)p.actions;        // (then no lane holds it: the first writes)
-                float lp = LN2 * (ya - known.log2_s);
-                if (exact || known.bad || xa < -LARGE) lp = known.logprob(xa, p);
-                if (none) lp = known.bad ? known.log2_s : 0.0f;
-                if (none ? lane == 0 : has) o.logprob[r] = lp;
+                    for (int i = 1; i < E; ++i) xa = a == i ? x[i] : xa;
+                    if ((unsigned)a < (unsigned)p.actions) lp = logprob(xa);
+                } else if ((unsigned)a < (unsigned)p.actions)
+                    lp = logprob(p.legal && !__ldg(p.legal + r * p.legal_stride + a) ? NONE : Of<TYPE>::get(static_cast<const typename Of<TYPE>::T*>(p.logits)[r * p.stride + a]));
+                o.logprob[r] = lp;
             }
         }
         if constexpr (TOP) {
             // the largest of the row's remaining values, of equal ones the lowest action, `top` times
-            if (known.bad) {
+            if constexpr (TYPE != CUDARL_F32) {                              // 16 bits of value and 16 of action: one integer
+                unsigned key[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[i] = NONE;
-            }
-            for (int k = 0; k < o.top; ++k) {
-                float high = x[0];
+                for (int i = 0; i < E; ++i) key[i] = x[i] > NONE && !known.bad ? order_key16<TYPE>(x[i], (unsigned)short_action<G, E, WIDE>(lane, i)) : 0u;
+                int* const top_actions = o.top_actions + r * o.top;
+                float* const top_logprobs = o.top_logprobs + r * o.top;
+                for (int k = 0; k < o.top; ++k) {
+                    unsigned best = key[0];
 #pragma unroll
-                for (int i = 1; i < E; ++i) high = fmaxf(high, x[i]);
+                    for (int i = 1; i < E; ++i) best = max(best, key[i]);
 #pragma unroll
-                for (int by = 1; by < G; by *= 2) high = fmaxf(high, __shfl_xor_sync(ALL, high, by));
-                int at = 0x7FFFFFFF;
+                    for (int by = 1; by < G; by *= 2) best = max(best, __shfl_xor_sync(ALL, best, by));
 #pragma unroll
-                for (int i = E - 1; i >= 0; --i) at = x[i] == high ? short_action<G, E, WIDE>(lane, i) : at;
+                    for (int i = 0; i < E; ++i) key[i] = key[i] == best ? 0u : key[i];
+                    if (write && lane == 0) {
+                        top_actions[k] = best ? (int)(0xFFFFu - (best & 0xFFFFu)) : -1;
+                        top_logprobs[k] = best ? logprob(key16_value<TYPE>(best)) : known.bad ? known.log2_s : NONE;
+                    }
+                }
+            } else {
+                if (known.bad) {
 #pragma unroll
-                for (int by = 1; by < G; by *= 2) at = min(at, __shfl_xor_sync(ALL, at, by));
-                const bool there = high > NONE;
+                    for (int i = 0; i < E; ++i) x[i] = NONE;
+                }
+                int* const top_actions = o.top_actions + r * o.top;
+                float* const top_logprobs = o.top_logprobs + r * o.top;
+                for (int k = 0; k < o.top; ++k) {
+                    float high = x[0];
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[i] = there && short_action<G, E, WIDE>(lane, i) == at ? NONE : x[i];
-                if (write && lane == 0) {
-                    o.top_actions[r * o.top + k] = there ? at : -1;
-                    o.top_logprobs[r * o.top + k] = known.bad ? known.log2_s : there ? known.logprob(high, p) : NONE;
+                    for (int i = 1; i < E; ++i) high = fmaxf(high, x[i]);
+#pragma unroll
+                    for (int by = 1; by < G; by *= 2) high = fmaxf(high, __shfl_xor_sync(ALL, high, by));
+                    int at = 0x7FFFFFFF;
+#pragma unroll
+                    for (int i = E - 1; i >= 0; --i) at = x[i] == high ? short_action<G, E, WIDE>(lane, i) : at;
+#pragma unroll
+                    for (int by = 1; by < G; by *= 2) at = min(at, __shfl_xor_sync(ALL, at, by));
+                    const bool there = high > NONE;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) x[i] = there && short_action<G, E, WIDE>(lane, i) == at ? NONE : x[i];
+                    if (write && lane == 0) {
+                        top_actions[k] = there ? at : -1;
+                        top_logprobs[k] = there ? logprob(high) : known.bad ? known.log2_s : NONE;
+                    }
                 }
             }
         }
@@ -340,19 +376,23 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
 // ------------------------------------------------------------------------------------------------------------------ parts of warps
 __device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float warp_min(float v) { float r; asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+// Has the bytes from `at` to `end` on their way to L2, 32 lanes a sector each at a time.
+__device__ __forceinline__ void fetch_ahead(const void* at, const void* end, unsigned lane) {
+    for (const char* a = static_cast<const char*>(at) + lane * 32u; a < static_cast<const char*>(end); a += 1024) asm volatile("prefetch.global.L2 [%0];" :: "l"(a));
+}
 // The 32 lanes' parts as one, in every lane.
 __device__ __forceinline__ void join_lanes(Part& p, float c, int lanes = 32) {
     rebase(p, warp_max(p.m), c);
     for (int by = lanes / 2; by; by /= 2) { p.s += __shfl_xor_sync(ALL, p.s, by); p.t += __shfl_xor_sync(ALL, p.t, by); }
 }
 // The `rank`-th largest of the lanes' values (1 .. 32).
-__device__ __forceinline__ float warp_ranked(float v, int rank, unsigned lane) {
-    float high = NONE;
-    for (int k = 0; k < rank; ++k) {
-        high = warp_max(v);
-        if (lane == (unsigned)__ffs((int)__ballot_sync(ALL, v == high)) - 1u) v = NONE;
+__device__ __forceinline__ float warp_ranked(float v, int rank) {
+    while (true) {
+        const float high = warp_max(v);
+        rank -= __popc(__ballot_sync(ALL, v == high));
+        if (rank <= 0 || high == NONE) return high;
+        v = v == high ? NONE : v;
     }
-    return high;
 }
 // A whole row by the threads of a team a second time, with exact differences: lane- and warp-wise parts of it (see below for where it is needed).
 template <int AT_ONCE, int TYPE, class F> __device__ __forceinline__ void each_chunk(const Row<TYPE>& row, int t, int threads, F f) {
@@ -511,7 +551,7 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
             if ((int)lane == i_row) mine = part;
             if constexpr (TOP) {
                 const bool bad = !(part.s == part.s);
-                const float bound = warp_ranked(own, o.top, lane);
+                const float bound = warp_ranked(own, o.top);
                 int n = 0;
                 if (bound > ABOVE_FLOOR && !bad) {
                     auto list = [&](float v, int j) {
@@ -638,6 +678,10 @@ __global__ void __launch_bounds__(T, (T == 128 && !MASKED ? 768 : 1024) / T) k_l
         if (AHEAD) load(0);
         for (int b = 0; b < batches; ++b) {
             if (!AHEAD) load(b);
+            if (T == 32 && b + 1 < batches) {                                // the next batch's bytes on their way meanwhile
+                const auto* const at = row.x + row.head + (b + 1) * BATCH * N;
+                fetch_ahead(at, at + min(BATCH, row.chunks - (b + 1) * BATCH) * N, lane);
+            }
             float x[UNROLL][N], bm = NONE;
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) take_chunk<TYPE, MASKED>(raw[u], legal[u], x[u], bm);
@@ -832,27 +876,17 @@ __global__ void __launch_bounds__(256) k_short_backward(Rows p, const float* gra
         const Part part = sum_short<G, E>(x, p.scale, y, e, exact);
         const Known known(part);
         const float A = -p.scale * (gl + gh * known.h), B = -p.scale * gh * LN2, share = __fdividef(1.0f, part.s);
-        // the taken action: 1 - p is the others' share
-        float others = 0.0f, ya = 0.0f, ea = 0.0f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const bool is = short_action<G, E, WIDE>(lane, i) == a;
-            others += is ? 0.0f : e[i];
-            ya = is ? y[i] : ya; ea = is ? e[i] : ea;
-        }
-#pragma unroll
-        for (int by = 1; by < G; by *= 2) others += __shfl_xor_sync(ALL, others, by);
-        const float ga = fmaf(p.scale * gl, others * share, fmaf(ea * share, B * (ya - known.log2_s), -p.scale * gh * known.h * ea * share));
+        const float more = p.scale * gl;                                     // of the action taken: scale gl (1 - p) is one product less p's
 #pragma unroll
         for (int i = 0; i < E; i += 2) {
             const Two lp2 = add2(two(y[i], y[i + 1]), two(-known.log2_s, -known.log2_s)), p2 = mul2(two(e[i], e[i + 1]), two(share, share));
-            apart(mul2(p2, fma2(two(B, B), lp2, two(A, A))), y[i], y[i + 1]);
+            apart(mul2(p2, fma2(two(B, B), lp2, two(A, A))), x[i], x[i + 1]);
         }
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            x[i] = taken && short_action<G, E, WIDE>(lane, i) == a ? ga : y[i];
-            if (known.nothing) x[i] = 0.0f;
-            if (known.bad) x[i] = known.log2_s;
+        for (int i = 0; i < E; ++i) x[i] += taken && short_action<G, E, WIDE>(lane, i) == a ? more : 0.0f;
+        if (known.nothing || known.bad) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = known.bad ? known.log2_s : 0.0f;
         }
         if (p.legal) {
             const unsigned char* legal = p.legal + r * p.legal_stride;

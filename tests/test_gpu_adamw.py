@@ -227,6 +227,26 @@ def test_many_tensors_and_a_large_one(pkg):
         check(net, before, 1, 0.01, 0.5 / (norm + 1e-6), seed=2)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_handles_at_once(pkg, bits):
+    """Two networks on two streams, and the same steps one after the other."""
+    nets = [Net(pkg, [70000, 300, 5001], "bf16", "bf16", True, bits, seed=k % 2) for k in range(4)]
+    opts = [pkg.AdamW(n.list(), state_bits=bits, seed=6, max_grad_norm=1.0) for n in nets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for k in range(2):
+            opts[k].step(0.01, stream=streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    for k in (2, 3):
+        for _ in range(20):
+            opts[k].step(0.01)
+    torch.cuda.synchronize()
+    for k in range(2):
+        for (a, _o, _n), (b, _o2, _n2) in zip(nets[k].all, nets[k + 2].all):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_no_tensors(pkg):
     opt = pkg.AdamW([])
     opt.step(0.1)
@@ -306,6 +326,7 @@ def test_tensors_are_refused(pkg):
     refused("lr_scale", lr_scale=-1.0)
     refused("aligned", param=net.tensors[0]["param"].data_ptr() + 2)
     refused("not device memory", master=torch.zeros(100).data_ptr())
+    refused("2\\^34", count=(1 << 34) + 1)                                   # (nothing of it is touched)
     t = net.list()[0]
     t.grad = None
     opt = pkg.AdamW([t])

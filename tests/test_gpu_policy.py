@@ -241,6 +241,58 @@ def test_many_rows_and_one_long_row(pkg, t):
         assert ((g.double() - eg).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n,v,top", [(1300, 1025, 3), (1300, 2500, 32), (1201, 5003, 8), (1184, 8192, 1), (310, 9001, 5), (700, 33000, 2), (80, 70001, 20), (2500, 300, 4), (9001, 700, 1),
+                                     (4099, 1024, 16), (30000, 33, 6), (5, 131072, 32)])
+def test_every_way_to_split_the_work(pkg, t, masked, n, v, top):
+    """Many rows and few of them, a warp, a block or a cluster each: against 64 bits on the device, with rows that nothing is left of among the others."""
+    gen = torch.Generator("cuda").manual_seed(n + v)
+    x = (torch.randn(n, v, device="cuda", generator=gen) * 3).to(TYPES[t])
+    legal = None
+    z = x.double() * float(np.float32(0.8))
+    if masked:
+        legal = torch.rand(n, v, device="cuda", generator=gen) < 0.4
+        legal[n // 2] = False
+        legal[3] = False
+        legal[3, v - 1] = True
+        z = z.masked_fill(~legal, -np.inf)
+        legal = legal.to(torch.uint8)
+    taken = torch.randint(0, v, (n,), device="cuda", dtype=torch.int32, generator=gen)
+    p, (lp, h, ta, tl, st), _keep = forward(pkg, x, t, taken, legal, 0.8, top, stats=True)
+    empty = torch.isinf(z).all(1)
+    logp = (z - torch.logsumexp(z, 1, keepdim=True)).masked_fill(empty[:, None], -np.inf)
+    pr = logp.exp()
+    e = (v / 32 + 70 + 3 * (12 + np.log(v))) * U
+    want = logp.gather(1, taken.long()[:, None])[:, 0]
+    assert torch.equal(torch.isinf(want), torch.isinf(lp[:n]))
+    fine = ~torch.isinf(want)
+    assert ((lp[:n] - want)[fine].abs() <= e + 4 * U * want[fine].abs()).all()
+    eh = -torch.nan_to_num(pr * logp, nan=0.0).sum(1)
+    assert ((h[:n] - eh).abs() <= e * (2 + eh)).all()
+    key = x.double() if legal is None else x.double().masked_fill(legal == 0, -np.inf)
+    best, at = torch.sort(key, dim=1, descending=True, stable=True)
+    at = at[:, :top].masked_fill(torch.isinf(best[:, :top]), -1)
+    assert torch.equal(ta[:n * top].view(n, top).long(), at)
+    wl = logp.gather(1, at.clamp(min=0)).masked_fill(at < 0, -np.inf)
+    tl = tl[:n * top].view(n, top)
+    assert torch.equal(torch.isinf(tl), torch.isinf(wl))
+    fine = ~torch.isinf(wl)
+    assert ((tl - wl)[fine].abs() <= e + 4 * U * wl[fine].abs()).all()
+    gl, gh = torch.randn(n, device="cuda", generator=gen), torch.randn(n, device="cuda", generator=gen)
+    g = torch.empty(n, v, dtype=TYPES[t], device="cuda")
+    pkg.policy_logprobs_backward(p, st.data_ptr(), gl.data_ptr(), gh.data_ptr(), g.data_ptr())
+    one = torch.zeros_like(pr).scatter_(1, taken.long()[:, None], 1.0)
+    lq = torch.where(pr > 0, logp, 0.0)
+    scale = float(np.float32(0.8))
+    eg = scale * (gl[:, None] * (one - pr) - gh[:, None] * pr * (lq + eh[:, None]))
+    eg[empty] = 0.0
+    if legal is not None:
+        eg[legal == 0] = 0.0
+    tol = scale * (gl.abs()[:, None] * pr + gh.abs()[:, None] * pr * (lq.abs() + eh[:, None] + 1)) * 2 * (e + 8 * U) + eg.abs() * (4 * U + plain.HALF_STEP[t]) + plain.TINY[t]
+    assert ((g.double() - eg).abs() <= tol).all()
+
+
 def test_rows_far_apart(pkg):
     """Offsets above 32 bits: three rows 2^31 values apart."""
     v, stride = 1003, (1 << 31) + 8

@@ -15,13 +15,14 @@ def text(pkg):
 
 
 def test_struct_sizes(pkg):
+    assert pkg.MAX_TOP == 32 and pkg.ADAMW_BLOCK == 256
     assert [C.sizeof(t) for t in (pkg.PolicyRows, pkg.AdamWTensor, pkg.AdamWConfig, pkg.AdamWStats)] == [72, 80, 56, 24]
 
 
 @pytest.mark.parametrize("kw,word", [
     (dict(struct_size=8), "struct_size"), (dict(type=3), "type"), (dict(type=-1), "type"), (dict(rows=-1), "rows"), (dict(actions=0), "actions"), (dict(actions=1 << 31), "actions"),
     (dict(row_stride=4), "row_stride"), (dict(row_stride=1 << 60), "strides"), (dict(rows=1 << 38, row_stride=1 << 38), "strides"), (dict(legal=A, legal_stride=4), "legal_stride"), (dict(legal=A, legal_stride=-1), "legal_stride"),
-    (dict(inv_temperature=0.0), "inv_temperature"), (dict(inv_temperature=-1.0), "inv_temperature"), (dict(inv_temperature=float("inf")), "inv_temperature"),
+    (dict(actions=(1 << 30) + 1), "actions"), (dict(inv_temperature=0.0), "inv_temperature"), (dict(inv_temperature=9e-7), "inv_temperature"), (dict(inv_temperature=2e6), "inv_temperature"), (dict(inv_temperature=-1.0), "inv_temperature"), (dict(inv_temperature=float("inf")), "inv_temperature"),
     (dict(inv_temperature=float("nan")), "inv_temperature"), (dict(logits=None), "logits"), (dict(logits=A + 2), "aligned")])
 def test_rows_are_refused(pkg, kw, word):
     lib = pkg.load()
