@@ -270,34 +270,39 @@ template <int TYPE, int COUNT> __device__ __forceinline__ void add_squares(doubl
 
 // Sum of squares of all gradients, in 64 bits and in an order that only the list of pieces and the grid make; the last block adds the blocks' sums.  A warp a
 // piece, 64 (32 bits) or 128 bytes a lane on their way at a time: as many conversions to 64 bits as take about two thirds of the time that the bytes take.
-__global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tensors, const Piece* __restrict__ pieces, unsigned n, Control* ctl, double* part, float grad_scale, float max_norm) {
+__global__ void __launch_bounds__(32 * WARPS, 4) k_grad_norm(const Tensor* tensors, const Piece* __restrict__ pieces, unsigned n, Control* ctl, double* part, bool spread, float grad_scale, float max_norm) {
     asm volatile("griddepcontrol.launch_dependents;");                       // the step's blocks may come as these go: they load before they wait for the norm
     double four[4] = {0.0, 0.0, 0.0, 0.0};                                   // (four sums in turn: additions of 64 bits take their time)
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, stride = gridDim.x * WARPS;
+    auto add_block = [&](const Tensor& t, long long at) {                    // one block, or what there is of it
+        Raw raw;
+        float g[8];
+        const int len = (int)min(8ll, t.count - at);
+        load8(raw, t.grad, t.grad_type, at, t.wide_grad && len == 8, len);
+        floats8(raw, t.grad_type, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) four[i % 4] = fma((double)g[i], (double)g[i], four[i % 4]);
+    };
     unsigned k = blockIdx.x * WARPS + warp;                                  // (no overflow: at most 2^26 pieces)
+    if (spread) {                                                            // few pieces: a warp a block
+        const Piece pc = pieces[blockIdx.x];
+        if (warp < pc.blocks) add_block(tensors[pc.tensor], (long long)(pc.block + warp) * BLOCK + lane * 8u);
+        k = n;
+    }
     Piece next = k < n ? pieces[k] : Piece{0u, 0u, 0u, 0u};
     for (; k < n; k += stride) {
         const Piece pc = next;
         if (k + stride < n) next = pieces[k + stride];
         const Tensor& t = tensors[pc.tensor];
         const int type = t.grad_type;
-        const void* const grad = t.grad;
-        const long long first = (long long)pc.block * BLOCK, at = first + lane * 8u, left = t.count - first;
-        if (t.wide_grad && left >= WARPS * BLOCK) {
+        const long long first = (long long)pc.block * BLOCK, at = first + lane * 8u;
+        if (t.wide_grad && t.count - first >= WARPS * BLOCK) {
             static_assert(WARPS == 8, "the blocks of a whole piece");
-            if (type == CUDARL_F32) { add_squares<CUDARL_F32, 4>(four, grad, at); add_squares<CUDARL_F32, 4>(four, grad, at + 4 * BLOCK); }
-            else if (type == CUDARL_BF16) add_squares<CUDARL_BF16, 8>(four, grad, at);
-            else add_squares<CUDARL_F16, 8>(four, grad, at);
-        } else {
-            for (unsigned u = 0; u < pc.blocks; ++u) {
-                Raw raw;
-                float g[8];
-                load8(raw, grad, type, at + u * BLOCK, false, (int)min(8ll, left - (long long)(u * BLOCK + lane * 8u)));
-                floats8(raw, type, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) four[i % 4] = fma((double)g[i], (double)g[i], four[i % 4]);
-            }
-        }
+            if (type == CUDARL_F32) { add_squares<CUDARL_F32, 4>(four, t.grad, at); add_squares<CUDARL_F32, 4>(four, t.grad, at + 4 * BLOCK); }
+            else if (type == CUDARL_BF16) add_squares<CUDARL_BF16, 8>(four, t.grad, at);
+            else add_squares<CUDARL_F16, 8>(four, t.grad, at);
+        } else
+            for (unsigned u = 0; u < pc.blocks; ++u) add_block(t, at + u * BLOCK);
     }
     double sum = block_sum((four[0] + four[1]) + (four[2] + four[3]));
     __shared__ bool last;
@@ -566,8 +571,8 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, o->cfg.device)) != cudaSuccess) return fail_cuda("cudaDeviceGetAttribute", e);
     const unsigned most = (unsigned)(sms * RESIDENT), blocks = o->pieces;
     o->grid = blocks < 1u ? 1u : blocks < most ? blocks : most;
-    const unsigned norm_most = (unsigned)(sms * 4), norm_blocks = (o->pieces + WARPS - 1) / WARPS;
-    o->norm_grid = norm_blocks < 1u ? 1u : norm_blocks < norm_most ? norm_blocks : norm_most;
+    const unsigned norm_most = (unsigned)(sms * 4);                          // a block of threads a piece where there are so few, else a warp
+    o->norm_grid = o->pieces < 1u ? 1u : o->pieces < norm_most ? o->pieces : norm_most;
     Control c;
     std::memset(&c, 0, sizeof c);
     c.step = o->cfg.step;
@@ -629,7 +634,7 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
         s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;
     }
     if (s.clipped) {
-        k_grad_norm<<<o->norm_grid, 32 * WARPS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, grad_scale, c.max_grad_norm);
+        k_grad_norm<<<o->norm_grid, 32 * WARPS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, o->norm_grid == o->pieces, grad_scale, c.max_grad_norm);
         if ((e = cudaGetLastError()) != cudaSuccess) return fail_cuda("cudarl_adamw_step", e);
     }
     cudaLaunchConfig_t launch = {};

@@ -859,57 +859,72 @@ struct Slope {
     }
 };
 
-// Short rows have their sums in a few instructions: they are taken again instead of the statistics, which are as long as such a row.
+// Short rows have their sums in a few instructions: they are taken again instead of the statistics, which are as long as such a row.  AT_ONCE rows of a thread have
+// their loads on their way together where a row is a single load.
 template <int TYPE, int G, int E, bool WIDE>
 __global__ void __launch_bounds__(256) k_short_backward(Rows p, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
     using O = Of<TYPE>;
+    constexpr int AT_ONCE = G == 1 && E == 4 ? 2 : 1, ROWS = 256 / G;
     const int lane = (int)threadIdx.x % G;
-    const long long step = (long long)gridDim.x * (256 / G);
-    for (long long first = (long long)blockIdx.x * (256 / G); first < p.rows; first += step) {
-        const long long mine = first + (int)threadIdx.x / G, r = mine < p.rows ? mine : p.rows - 1;
-        float x[E], y[E], e[E];
-        load_short<TYPE, G, E, WIDE>(p, r, lane, x);
-        const int a = p.taken ? __ldg(p.taken + r) : -1;
-        const bool taken = (unsigned)a < (unsigned)p.actions;
-        const float gl = taken && grad_logprob ? __ldg(grad_logprob + r) : 0.0f, gh = grad_entropy ? __ldg(grad_entropy + r) : 0.0f;
-        bool exact;
-        const Part part = sum_short<G, E>(x, p.scale, y, e, exact);
-        const Known known(part);
-        const float A = -p.scale * (gl + gh * known.h), B = -p.scale * gh * LN2, share = __fdividef(1.0f, part.s);
-        const float more = p.scale * gl;                                     // of the action taken: scale gl (1 - p) is one product less p's
+    const long long step = (long long)gridDim.x * ROWS * AT_ONCE;
+    for (long long first = (long long)blockIdx.x * ROWS * AT_ONCE; first < p.rows; first += step) {
+        float xs[AT_ONCE][E], gls[AT_ONCE], ghs[AT_ONCE];
+        int as[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const Two lp2 = add2(two(y[i], y[i + 1]), two(-known.log2_s, -known.log2_s)), p2 = mul2(two(e[i], e[i + 1]), two(share, share));
-            apart(mul2(p2, fma2(two(B, B), lp2, two(A, A))), x[i], x[i + 1]);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const long long mine = first + u * ROWS + (int)threadIdx.x / G, r = mine < p.rows ? mine : p.rows - 1;
+            load_short<TYPE, G, E, WIDE>(p, r, lane, xs[u]);
+            as[u] = p.taken ? __ldg(p.taken + r) : -1;
+            gls[u] = grad_logprob ? __ldg(grad_logprob + r) : 0.0f;
+            ghs[u] = grad_entropy ? __ldg(grad_entropy + r) : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] += taken && short_action<G, E, WIDE>(lane, i) == a ? more : 0.0f;
-        if (known.nothing || known.bad) {
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const long long mine = first + u * ROWS + (int)threadIdx.x / G, r = mine < p.rows ? mine : p.rows - 1;
+            float (&x)[E] = xs[u];
+            float y[E], e[E];
+            const int a = as[u];
+            const bool taken = (unsigned)a < (unsigned)p.actions;
+            const float gl = taken ? gls[u] : 0.0f, gh = ghs[u];
+            bool exact;
+            const Part part = sum_short<G, E>(x, p.scale, y, e, exact);
+            const Known known(part);
+            const float A = -p.scale * (gl + gh * known.h), B = -p.scale * gh * LN2, share = __fdividef(1.0f, part.s);
+            const float more = p.scale * gl;                                 // of the action taken: scale gl (1 - p) is one product less p's
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = known.bad ? known.log2_s : 0.0f;
-        }
-        if (p.legal) {
-            const unsigned char* legal = p.legal + r * p.legal_stride;
-#pragma unroll
-            for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions && !__ldg(legal + j)) x[i] = 0.0f; }
-        }
-        if (mine >= p.rows) continue;                                        // (a whole team: nothing of it is waited for)
-        auto* at = static_cast<typename O::T*>(grad) + r * grad_stride;
-        constexpr int BYTES = E * (int)sizeof(typename O::T);
-        if (WIDE && lane * E + E <= p.actions) {
-            if constexpr (BYTES == 8 && TYPE != CUDARL_F32) *reinterpret_cast<uint2*>(at + lane * E) = make_uint2(Chunk<TYPE>::two16(x[0], x[1]), Chunk<TYPE>::two16(x[2], x[3]));
-            else if constexpr (BYTES >= 16) {
-#pragma unroll
-                for (int k = 0; k < BYTES / 16; ++k) {
-                    float part[Chunk<TYPE>::N];
-#pragma unroll
-                    for (int i = 0; i < Chunk<TYPE>::N; ++i) part[i] = x[k * Chunk<TYPE>::N + i];
-                    reinterpret_cast<uint4*>(at + lane * E)[k] = Chunk<TYPE>::pack(part);
-                }
+            for (int i = 0; i < E; i += 2) {
+                const Two lp2 = add2(two(y[i], y[i + 1]), two(-known.log2_s, -known.log2_s)), p2 = mul2(two(e[i], e[i + 1]), two(share, share));
+                apart(mul2(p2, fma2(two(B, B), lp2, two(A, A))), x[i], x[i + 1]);
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions) at[j] = O::put(x[i]); }
+            for (int i = 0; i < E; ++i) x[i] += taken && short_action<G, E, WIDE>(lane, i) == a ? more : 0.0f;
+            if (known.nothing || known.bad) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[i] = known.bad ? known.log2_s : 0.0f;
+            }
+            if (p.legal) {
+                const unsigned char* legal = p.legal + r * p.legal_stride;
+#pragma unroll
+                for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions && !__ldg(legal + j)) x[i] = 0.0f; }
+            }
+            if (mine >= p.rows) continue;                                    // (a whole team: nothing of it is waited for)
+            auto* at = static_cast<typename O::T*>(grad) + r * grad_stride;
+            constexpr int BYTES = E * (int)sizeof(typename O::T);
+            if (WIDE && lane * E + E <= p.actions) {
+                if constexpr (BYTES == 8 && TYPE != CUDARL_F32) *reinterpret_cast<uint2*>(at + lane * E) = make_uint2(Chunk<TYPE>::two16(x[0], x[1]), Chunk<TYPE>::two16(x[2], x[3]));
+                else if constexpr (BYTES >= 16) {
+#pragma unroll
+                    for (int k = 0; k < BYTES / 16; ++k) {
+                        float values[Chunk<TYPE>::N];
+#pragma unroll
+                        for (int i = 0; i < Chunk<TYPE>::N; ++i) values[i] = x[k * Chunk<TYPE>::N + i];
+                        reinterpret_cast<uint4*>(at + lane * E)[k] = Chunk<TYPE>::pack(values);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) { const int j = short_action<G, E, WIDE>(lane, i); if (j < p.actions) at[j] = O::put(x[i]); }
+            }
         }
     }
 }
@@ -1088,7 +1103,7 @@ cudaError_t launch_short(const Rows& p, const Outputs& o, cudaStream_t st) {
 struct BackwardArgs { const float4* stats; const float* gl; const float* gh; void* grad; long long stride; };
 template <int TYPE, int G, int E, bool WIDE>
 cudaError_t launch_short(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
-    k_short_backward<TYPE, G, E, WIDE><<<blocks_of(p.rows, 256 / G), 256, 0, st>>>(p, b.gl, b.gh, b.grad, b.stride);
+    k_short_backward<TYPE, G, E, WIDE><<<blocks_of(p.rows, 256 / G * (G == 1 && E == 4 ? 2 : 1)), 256, 0, st>>>(p, b.gl, b.gh, b.grad, b.stride);
     return cudaGetLastError();
 }
 // Rows of up to SHORT_ACTIONS actions, either way (a call's outputs or a gradient's arguments).
