@@ -3,6 +3,9 @@
 // The handle keeps on the device: the list of the tensors, a list of the pieces of them that a block of threads takes at a time (up to eight blocks of 256 values,
 // a block being what one scale of the 8-bit moments is for), and the step count with what depends on it.  Nothing of a step comes from the host but lr and grad_scale, so a
 // captured step counts on.
+//
+// What bounds it (B200, kernels alone): with 32-bit moments the memory: 150M values of bf16 weights with masters, 28 bytes each, 695 us = 6.05 TB/s, 92 % of a copy's rate.
+// With 8-bit moments, 16 bytes a value, the instructions: 555 for a warp's 256 values, 141 us for 40M (4.2 TB/s); 200M with the norm 734 us.
 #include "async_copy.cuh"
 #include "caller_arrays.cuh"
 #include "rules.cuh"

@@ -3,7 +3,11 @@
 // Row x, legal actions L, scale = 1 / temperature, m = max x.  In base 2, with c = scale log2(e):
 //   y = x c - m c <= 0,   S = sum 2^y,   log2 p = y - log2 S,   H = ln 2 (log2 S - (sum y 2^y) / S)      (both terms >= 0: nothing cancels)
 //   dx_j = scale (gl ([j = taken] - p_j) - gH p_j (ln p_j + H))
-// What a row leaves for its gradient: {m, log2 S, H}.
+// What a row of more than 128 actions leaves for its gradient: {m, log2 S, H}.
+//
+// What bounds it (B200, times of the kernels alone): long rows the memory and, a step behind, the exponentials (16 a cycle and SM): 4096 x 131072 bf16, 1.07 GB, 178 us =
+// 6.0 TB/s without alternatives, 207 us with 5; its gradient, 2047 x 65537, 0.54 GB, 88 us = 6.1 TB/s.  Short rows the instructions that are made once a row:
+// 4,194,304 x 4 fp32 26.6 us forward (2.5 TB/s of logits, 4.4 with the actions and the results), gradient 37 us.
 //
 // y is one fused multiply-add with m c rounded once: an error of m c multiplies all 2^y of the row alike and leaves p as it is, so long as every
 // use takes the same m c.  Minus infinity, masked places and whatever is below FLOOR count as FLOOR (2^y is 0 there all the same), so y 2^y needs no
@@ -227,7 +231,8 @@ __device__ __forceinline__ void write_top(const Outputs& o, const Rows& p, const
 }
 
 // ------------------------------------------------------------------------------------------------------------------ short rows
-// G lanes a row, E values a lane in registers: up to G E actions.  WIDE: a lane has neighbouring values and moves them at once, which takes rows that are aligned
+// G lanes a row, E values a lane in registers: up to G E actions (100 of them, 500,000 rows of bf16: 61 us, gradient 90; as a warp a row 109 and 180; from 129 on the
+// two are alike without alternatives and 16 lanes the slower with 20 of them: 883 against 586 us for 500,000 x 256 fp32).  WIDE: a lane has neighbouring values and moves them at once, which takes rows that are aligned
 // to that; else neighbouring lanes have neighbouring values, so that what a warp reads or writes at a time lies together.
 template <int G, int E, bool WIDE> __device__ __forceinline__ int short_action(int lane, int i) { return WIDE ? lane * E + i : lane + G * i; }
 
@@ -481,7 +486,9 @@ template <int TYPE> __device__ __forceinline__ void add_chunk(const float (&x)[C
 // A warp a row, the whole row in registers: CHUNKS pieces of 16 bytes a lane, and an end.  What is
 // scalar in a row -- the taken action's logit, logarithm, quotient, addresses, the writes -- is done for up to 32 consecutive rows at a time, a lane each.
 // The alternatives: the `top`-th largest of the lanes' maxima is a bound that `top` values reach; what reaches it is listed, and each of those counts how many
-// are larger.
+// are larger.  65,536 x 257 fp32: 26 us (208 instructions a row), with a mask 40 (310), with a mask and 4 alternatives 66 (611): it is the instructions that bound
+// it.  (100,000 x 1000 fp32 with 4 alternatives 119 us, by the kernel for long rows 150; without 76 and 72.  Loading the next row into registers ahead, or having it
+// fetched to L2, made it slower: 92 and 78 us.)
 constexpr int WARP_KEYS = 64, GROUP_KEYS = 128;
 // Blocks on an SM for which the registers suffice.
 constexpr int warp_blocks(int values) { return values <= 8 ? 5 : values <= 16 ? 4 : 3; }
@@ -602,13 +609,16 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
 }
 
 // ------------------------------------------------------------------------------------------------------------------ long rows
-// T threads a row, or the blocks of a cluster for few rows.  A thread takes batches of UNROLL chunks; a batch costs one maximum and one rebasing of the thread's
+// T threads a row: a warp, 128, or the blocks of a cluster for few rows (which: launch_rows).  A thread takes batches of UNROLL chunks; a batch costs one maximum and one rebasing of the thread's
 // sums.  The threads' parts are joined by shuffles, in shared memory, and over the cluster in the other blocks' shared memory.
 //
 // Alternatives: the maximum of every batch (of every GROUP of batches, for very long rows) is kept in shared memory.  32 of the threads' maxima, the largest of each
 // warp, are values of the row, so the `top`-th largest of them is a bound that `top` values reach.  Only batches that reach it are read again -- a few dozen --
 // and of what reaches the bound there each counts how many are larger.  Where too much does (rows of equal values) or too little (fewer than `top` values above
 // FLOOR), every value of the row is gone through again, each warp with its 32 best in registers.
+//
+// With 128 threads the next batch is loaded ahead into registers (4096 x 131072 bf16: 179 us, without 195; a ring of bulk copies by one more warp: 186 to 210, and 262
+// to 300 with alternatives, whose second look then waits for the copies' place).
 constexpr int UNROLL = 4,  TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
 
 template <int T> struct Shared {
@@ -1176,11 +1186,13 @@ cudaError_t launch_rows(const Rows& p, const Outputs& o, int sms, cudaStream_t s
     if (v <= 256) return launch_warp<TYPE, 256>(p, o, sms, st);
     if (v <= 512) return launch_warp<TYPE, 512>(p, o, sms, st);
     if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, o, sms, st);
-    // a cluster for each row where there are too few rows to occupy the GPU, as long as each block still gets half a batch
+    // a cluster for each row where there are too few rows to occupy the GPU, as long as each block still gets a batch (bf16, 20 alternatives, 1 / 2 / 4 / 8 blocks a
+    // row: 1 x 131072 32 / 20 / 16 / 14 us, 74 rows 34 / 21 / 19 / 25, 200 rows 34 / 26 / 32 / 40)
     int blocks = 1;
     while (blocks < 8 && p.rows * blocks < 2ll * sms && (long long)v >= 256ll * Chunk<TYPE>::N * UNROLL * blocks) blocks *= 2;
     if (blocks > 1) return launch_long<TYPE, 256>(p, o, blocks, st);
-    // a warp for each row where there are enough of them to occupy the GPU and what is done once a row weighs more than the wait for a batch
+    // a warp for each row where there are enough of them to occupy the GPU and what is done once a row weighs more than the wait for a batch (a warp / 128 threads:
+    // 8192 x 8192 bf16, 4 alternatives 44 / 61 us, 20000 x 2500 f16 53 / 113; 600 x 30000 fp32 50 / 24, 2047 x 65537 bf16 71 / 57)
     if (v <= 8192 && p.rows >= 8ll * sms) return launch_long<TYPE, 32>(p, o, 1, st);
     return launch_long<TYPE, 128>(p, o, 1, st);
 }

@@ -254,7 +254,8 @@ typedef struct cudarl_policy_rows {
     int32_t  reserved0;
 } cudarl_policy_rows;
 
-/* logprob[rows]: of the action taken.  entropy[rows]: in nats.  stats[4*rows], 16-byte aligned: what the backward call reads.
+/* logprob[rows]: of the action taken.  entropy[rows]: in nats.  stats[4*rows], 16-byte aligned: what the backward call reads (rows of up to
+ * 128 actions need none: it is left as it is).
  * top_actions / top_logprobs [rows*top]: the `top` (0 .. CUDARL_MAX_TOP) most probable actions in falling order, of equal
  * logits the lowest action first; places that no action is left for hold -1 and minus infinity.  Any output may be NULL (the
  * two top arrays only together with top = 0).
