@@ -86,7 +86,7 @@ struct Known {
     bool nothing, bad;                                                       // no action has any probability; a NaN or plus infinity is among them
     __device__ __forceinline__ Known(const Part& p) {
         nothing = p.s == 0.0f; bad = !(p.s == p.s);
-        m = p.m; log2_s = __log2f(p.s); h = nothing ? 0.0f : LN2 * (log2_s - __fdividef(p.t, p.s));      // (s is 1 or more: both are good to some 2^-22)
+        m = p.m; log2_s = __log2f(p.s); h = nothing ? 0.0f : max_nan(LN2 * (log2_s - __fdividef(p.t, p.s)), 0.0f);      // (s is 1 or more: both are good to some 2^-22)
     }
     // Log probability of an action with this logit.
     __device__ __forceinline__ float logprob(float x, const Rows& p) const {
@@ -94,7 +94,7 @@ struct Known {
         if (x == NONE || nothing) return NONE;
         const float c = p.scale * LOG2E;
         if (!(fabsf(x) < LARGE && is_usual(m, c))) return (x - m) * p.scale - LN2 * log2_s;
-        return LN2 * (fmaf(x, c, -(m * c)) - log2_s);
+        return fminf(LN2 * (fmaf(x, c, -(m * c)) - log2_s), 0.0f);
     }
     __device__ __forceinline__ void write(const Outputs& o, long long r) const {
         if (o.entropy) o.entropy[r] = h;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
         const Known known(sum_short<G, E>(x, p.scale, y, e, exact));
         const bool rare = exact || known.bad;
         const float c = p.scale * LOG2E, base = -(known.m * c);
-        auto logprob = [&](float v) { return rare || v < -LARGE ? known.logprob(v, p) : LN2 * (fmaf(v, c, base) - known.log2_s); };
+        auto logprob = [&](float v) { return rare || v < -LARGE ? known.logprob(v, p) : fminf(LN2 * (fmaf(v, c, base) - known.log2_s), 0.0f); };
         if (write && lane == 0) {
             if (o.entropy) o.entropy[r] = known.h;
             if (o.logprob) {
@@ -381,9 +381,9 @@ __global__ void __launch_bounds__(256) k_short(Rows p, Outputs o) {
 // ------------------------------------------------------------------------------------------------------------------ parts of warps
 __device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float warp_min(float v) { float r; asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
-// Has the bytes from `at` to `end` on their way to L2, 32 lanes a sector each at a time.
-__device__ __forceinline__ void fetch_ahead(const void* at, const void* end, unsigned lane) {
-    for (const char* a = static_cast<const char*>(at) + lane * 32u; a < static_cast<const char*>(end); a += 1024) asm volatile("prefetch.global.L2 [%0];" :: "l"(a));
+// Has the bytes from `at` to `end` on their way to L2, a sector a thread at a time.
+__device__ __forceinline__ void fetch_ahead(const void* at, const void* end, int t, int threads) {
+    for (const char* a = static_cast<const char*>(at) + t * 32; a < static_cast<const char*>(end); a += threads * 32) asm volatile("prefetch.global.L2 [%0];" :: "l"(a));
 }
 // The 32 lanes' parts as one, in every lane.
 __device__ __forceinline__ void join_lanes(Part& p, float c, int lanes = 32) {
@@ -688,9 +688,11 @@ __global__ void __launch_bounds__(T, (T == 128 && !MASKED ? 768 : 1024) / T) k_l
         if (AHEAD) load(0);
         for (int b = 0; b < batches; ++b) {
             if (!AHEAD) load(b);
-            if (T == 32 && b + 1 < batches) {                                // the next batch's bytes on their way meanwhile
-                const auto* const at = row.x + row.head + (b + 1) * BATCH * N;
-                fetch_ahead(at, at + min(BATCH, row.chunks - (b + 1) * BATCH) * N, lane);
+            if (!AHEAD && b + 1 < batches) {                                 // the next batch's bytes on their way to L2 meanwhile
+                const int k = ((b + 1) * blocks + rank) * BATCH, left = min(BATCH, row.chunks - k) * N;
+                const auto* const at = row.x + row.head + k * N;
+                fetch_ahead(at, at + left, t, T);
+                if (MASKED) fetch_ahead(row.legal + row.head + k * N, row.legal + row.head + k * N + left, t, T);
             }
             float x[UNROLL][N], bm = NONE;
 #pragma unroll

@@ -62,6 +62,7 @@ def check_forward(pkg, x, t, taken, legal=None, scale=1.0, top=0, stride=None, o
     assert (lp[n:] == 77).all() and (h[n:] == 77).all() and (ta[n * top:] == 77).all() and (tl[n * top:] == 77).all()
     assert taken is not None or (lp == 77).all()
     ta, tl = ta[:n * top].reshape(n, top), tl[:n * top].reshape(n, top)
+    assert not (lp[:n] > 0).any() and not (h[:n] < 0).any() and not (tl > 0).any()
     e = (v / 32 + 70 + 3 * (12 + np.log(v))) * U
     if taken is not None:
         close(lp[:n], elp, e + 4 * U * np.abs(elp))
