@@ -1034,8 +1034,8 @@ template <int TYPE, bool MASKED>
 __global__ void __launch_bounds__(256) k_long_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
     using C = Chunk<TYPE>;
     using O = Of<TYPE>;
-    constexpr int N = C::N, T = 256;
-    const int t = (int)threadIdx.x;
+    constexpr int N = C::N;
+    const int t = (int)threadIdx.x, T = (int)blockDim.x;
     for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const auto* x = static_cast<const typename O::T*>(p.logits) + r * p.stride;
         auto* g = static_cast<typename O::T*>(grad) + r * grad_stride;
@@ -1209,10 +1209,12 @@ cudaError_t launch_backward(const Rows& p, const BackwardArgs& b, int sms, cudaS
     if (v <= 256) return launch_warp<TYPE, 256>(p, b, sms, st);
     if (v <= 512) return launch_warp<TYPE, 512>(p, b, sms, st);
     if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, b, sms, st);
-    const int each = 256 * UNROLL * Chunk<TYPE>::N;
-    const dim3 grid((unsigned)((v + each - 1) / each), (unsigned)(p.rows < 65535 ? p.rows : 65535));
-    if (p.legal) k_long_backward<TYPE, true><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
-    else k_long_backward<TYPE, false><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
+    // as few pieces a row as 256 threads a block allow, and no more threads in a block than a piece has work for
+    const int chunks = v / Chunk<TYPE>::N, pieces = (chunks + 256 * UNROLL - 1) / (256 * UNROLL), each = (chunks + pieces * UNROLL - 1) / (pieces * UNROLL);
+    const int threads = each <= 64 ? 64 : (each + 31) / 32 * 32;
+    const dim3 grid((unsigned)pieces, (unsigned)(p.rows < 65535 ? p.rows : 65535));
+    if (p.legal) k_long_backward<TYPE, true><<<grid, threads, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
+    else k_long_backward<TYPE, false><<<grid, threads, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
     return cudaGetLastError();
 }
 
