@@ -618,7 +618,8 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
 // FLOOR), every value of the row is gone through again, each warp with its 32 best in registers.
 //
 // With 128 threads the next batch is loaded ahead into registers (4096 x 131072 bf16: 179 us, without 195; a ring of bulk copies by one more warp: 186 to 210, and 262
-// to 300 with alternatives, whose second look then waits for the copies' place).
+// to 300 with alternatives, whose second look then waits for the copies' place).  Where the registers do not suffice for that it is fetched to L2 (with / without:
+// 30000 x 4096 fp32 76 / 79 us, 20000 x 2500 f16, 4 alternatives 51 / 53).
 constexpr int UNROLL = 4,  TABLE_ROWS = 32, LIST = 192, CANDIDATES = 256;
 
 template <int T> struct Shared {
@@ -1030,8 +1031,9 @@ __global__ void __launch_bounds__(256, warp_blocks(CHUNKS * Chunk<TYPE>::N)) k_w
 
 // Long rows: a block takes UNROLL chunks a thread of a piece of a row; chunks begin where the gradient's address is aligned, and the logits are read in the same
 // chunks where their address is too, else one by one.
+constexpr int PIECE_THREADS = 128;
 template <int TYPE, bool MASKED>
-__global__ void __launch_bounds__(256) k_long_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
+__global__ void __launch_bounds__(PIECE_THREADS) k_long_backward(Rows p, const float4* stats, const float* grad_logprob, const float* grad_entropy, void* grad, long long grad_stride) {
     using C = Chunk<TYPE>;
     using O = Of<TYPE>;
     constexpr int N = C::N;
@@ -1209,8 +1211,9 @@ cudaError_t launch_backward(const Rows& p, const BackwardArgs& b, int sms, cudaS
     if (v <= 256) return launch_warp<TYPE, 256>(p, b, sms, st);
     if (v <= 512) return launch_warp<TYPE, 512>(p, b, sms, st);
     if (v <= WARP_ACTIONS) return launch_warp<TYPE, 1024>(p, b, sms, st);
-    // as few pieces a row as 256 threads a block allow, and no more threads in a block than a piece has work for
-    const int chunks = v / Chunk<TYPE>::N, pieces = (chunks + 256 * UNROLL - 1) / (256 * UNROLL), each = (chunks + pieces * UNROLL - 1) / (pieces * UNROLL);
+    // as few pieces a row as PIECE_THREADS a block allow, and no more threads in a block than a piece has work for (always 256 threads / as here: 20000 x 2500 f16
+    // 67 / 43 us, 40000 x 1500 bf16 113 / 50; at most 256 / 128: 20000 x 6000 bf16 86 / 82, 10000 x 9000 masked 105 / 86, 20000 x 2500 fp32 63.5 / 67.6)
+    const int chunks = v / Chunk<TYPE>::N, most = PIECE_THREADS * UNROLL, pieces = (chunks + most - 1) / most, each = (chunks + pieces * UNROLL - 1) / (pieces * UNROLL);
     const int threads = each <= 64 ? 64 : (each + 31) / 32 * 32;
     const dim3 grid((unsigned)pieces, (unsigned)(p.rows < 65535 ? p.rows : 65535));
     if (p.legal) k_long_backward<TYPE, true><<<grid, threads, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
