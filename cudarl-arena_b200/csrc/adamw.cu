@@ -30,7 +30,8 @@ struct Tensor {
     float lr_scale, decay;
     unsigned char param_type, grad_type;
     unsigned char wide;                       // every array but the gradient begins at an address that bulk copies can start at and eight values can be stored to at once
-    unsigned char wide_grad;                  // the gradient does
+    unsigned char copied_grad;                // bulk copies of the gradient can start where it begins (16 bytes) ...
+    unsigned char wide_grad;                  // ... and eight of its values can be loaded at once (32 bytes for those of 32 bits)
 };
 struct Piece { unsigned tensor, block, blocks, number; };   // `blocks` blocks (1 .. WARPS) of a tensor from its block `block` on, which is number `number` of all
 
@@ -191,7 +192,7 @@ template <int BITS> __device__ __noinline__ void copy_pieces(Ring<BITS>& ring, c
         view.moment1 = moved(t.moment1, of_m); view.moment2 = moved(t.moment2, of_m);
         view.scale1 = t.scale1 + pc.block; view.scale2 = t.scale2 + pc.block;
         view.values = (unsigned)min(t.count - first, (long long)(WARPS * BLOCK)); view.blocks = pc.blocks; view.number = pc.number;
-        view.copied = t.wide && t.wide_grad ? view.values / BLOCK : 0u;
+        view.copied = t.wide && t.copied_grad ? view.values / BLOCK : 0u;
         view.lr_scale = t.lr_scale; view.decay = t.decay;
         view.grad_type = t.grad_type; view.param_type = t.param_type; view.weight_type = t.master ? CUDARL_F32 : t.param_type;
         view.wide = t.wide;
@@ -529,6 +530,15 @@ int check_tensor(const cudarl_adamw_tensor& t, int bits, CallerArrays& arrays) {
     return 0;
 }
 
+bool sixteen(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool eight(const void* p, size_t value) { return reinterpret_cast<uintptr_t>(p) % (8 * value) == 0; }
+
+void place_gradient(Tensor& t, const void* grad) {
+    t.grad = grad;
+    t.copied_grad = sixteen(grad);
+    t.wide_grad = eight(grad, type_bytes(t.grad_type));
+}
+
 void note_gradients(cudarl_adamw* o) {
     o->gradients = true;
     for (const Tensor& t : o->tensors) o->gradients = o->gradients && (t.grad || t.count == 0);
@@ -553,12 +563,10 @@ int fill(cudarl_adamw* o, int32_t count, const cudarl_adamw_tensor* tensors) {
         const cudarl_adamw_tensor& t = tensors[i];
         const int rc = check_tensor(t, o->cfg.state_bits, arrays);
         if (rc) return rc;
-        Tensor d{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.lr_scale, t.weight_decay, (unsigned char)t.param_type, (unsigned char)t.grad_type, 0, 0};
-        auto eight = [](const void* p, size_t value) { return reinterpret_cast<uintptr_t>(p) % (8 * value) == 0; };
-        auto sixteen = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+        Tensor d{t.param, t.grad, t.master, t.moment1, t.moment2, t.scale1, t.scale2, (long long)t.count, t.lr_scale, t.weight_decay, (unsigned char)t.param_type, (unsigned char)t.grad_type, 0, 0, 0};
         const size_t moment = o->cfg.state_bits == 8 ? 1 : 4;
         d.wide = eight(t.param, type_bytes(t.param_type)) && eight(t.master, 4) && sixteen(t.moment1) && sixteen(t.moment2) && eight(t.moment1, moment) && eight(t.moment2, moment);
-        d.wide_grad = sixteen(t.grad);
+        place_gradient(d, t.grad);
         o->tensors.push_back(d);
         const int64_t blocks = (t.count + BLOCK - 1) / BLOCK;
         if (number + blocks > (1ll << 26)) return fail_global(-1, "more than 2^34 values in one handle");
@@ -674,8 +682,7 @@ extern "C" int cudarl_adamw_set_gradients(cudarl_adamw* o, const void* const* gr
     }
     for (size_t i = 0; i < o->tensors.size(); ++i) {
         Tensor& t = o->tensors[i];
-        t.grad = grads[i];
-        t.wide_grad = reinterpret_cast<uintptr_t>(t.grad) % 16 == 0;
+        place_gradient(t, grads[i]);
     }
     note_gradients(o);
     // the copy is from pageable memory: it has been taken from there when the call returns

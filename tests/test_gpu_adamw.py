@@ -149,6 +149,28 @@ def test_alignments(pkg, bits, offset):
 
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("grad", TYPES)
+@pytest.mark.parametrize("offset", [1, 2, 4, 8, 12])
+@pytest.mark.parametrize("sizes", [[4097, 300, 8, 1500], [1500000, 2048, 7]])
+def test_the_norm_of_gradients_at_every_alignment(pkg, bits, grad, offset, sizes):
+    """Four values are 16 bytes in, where a bulk copy of them can start and eight of 32 bits cannot be loaded at once; few pieces, and more than blocks."""
+    net = Net(pkg, sizes, "f32", grad, False, bits, size=1e-3)
+    for t, n in zip(net.tensors, sizes):                                     # only the gradient lies oddly
+        whole = torch.full((n + offset + 40,), 77, device="cuda").to(TYPES[grad])
+        whole[offset:offset + n] = t["grad"]
+        t["grad"] = whole[offset:offset + n]
+        net.all.append((whole, offset, n))
+    before = net.snapshot()
+    norm = np.sqrt(sum((g ** 2).sum() for _w, g, _m, _v in before))
+    most = float(np.float32(norm / 3))
+    opt = pkg.AdamW(net.list(), state_bits=bits, max_grad_norm=most)
+    opt.step(0.01)
+    check(net, before, 1, 0.01, most / (norm + 1e-6))
+    assert abs(opt.get_stats().grad_norm - norm) <= 1e-12 * norm
+    net.untouched()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grad", TYPES)
 def test_clipping(pkg, bits, grad):
     net = Net(pkg, [100, 20000, 1, 777], grad=grad, bits=bits)
     for most, scale in ((1.0, 1.0), (1e6, 0.5), (0.25, -2.0)):
