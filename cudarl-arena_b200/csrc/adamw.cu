@@ -11,6 +11,7 @@
 #include "rules.cuh"
 #include <cuda_fp8.h>
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -351,13 +352,17 @@ __device__ __forceinline__ Two divide2(Two a, float b, float by) {
     return fma2(fma2(q, negative2(b), a), by2, q);
 }
 __device__ __forceinline__ float reciprocal(float b) { const float r = reciprocal_fast(b); return fmaf(r, fmaf(-b, r, 1.0f), r); }
-// Zero stays zero; below 2^-100 the root is only about right.
+// Zero stays zero (its reciprocal root is infinite, and is made a number).  Below 2^-100 the remainder is not exact any more and the root is what the approximation
+// and its product are, 2^-22 of itself off at most; an infinite value gives NaN and is seen to behind this (one test a lane: the reciprocal root is zero there).
 __device__ __forceinline__ Two root2(Two v) {
     float a, b;
-    apart(add2(v, two(1e-37f, 1e-37f)), a, b);
-    const Two r = two(reciprocal_root_fast(a), reciprocal_root_fast(b)), q = mul2(v, r), rest = fma2(mul2(q, two(-1.0f, -1.0f)), q, v);
+    apart(v, a, b);
+    const Two r = two(fminf(reciprocal_root_fast(a), FLT_MAX), fminf(reciprocal_root_fast(b), FLT_MAX)), q = mul2(v, r), rest = fma2(mul2(q, two(-1.0f, -1.0f)), q, v);
     return fma2(rest, mul2(r, two(0.5f, 0.5f)), q);
 }
+// What an infinite root is kept as in 8 bits: its square is infinite again, so that the value stays where it is, as with moments of 32 bits -- and its block's scale is a
+// number (an infinite one would make NaN of the block's zeros).  Roots of floats end below 2^64.
+constexpr float INFINITE_ROOT = 36893488147419103232.0f;                     // 2^65
 
 // A block of threads takes a piece, a warp a block of it, a lane eight values.  Every product and sum of the moments is rounded by itself, and the roots and
 // quotients that become codes are correctly rounded (but for one in thousands, off by the last bit): codes do not depend on what a compiler fuses.
@@ -417,18 +422,27 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
                 apart(mul2(r, r), v[i], v[i + 1]);
             }
         }
-        float root[8];
+        float root[8], top2 = 0.0f;
         const Two one2 = two(s.one, s.one);                                  // (a product by a one that the compiler does not know, plus: a sum that it cannot fuse with the product before)
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             const Two gi = mul2(two(g[i], g[i + 1]), two(scale, scale));
             const Two mi = fma2(mul2(two(s.beta1, s.beta1), two(m[i], m[i + 1])), one2, mul2(two(s.rest1, s.rest1), gi));
-            const Two vi = fma2(mul2(two(s.beta2, s.beta2), two(v[i], v[i + 1])), one2, mul2(mul2(two(s.rest2, s.rest2), gi), gi)), ri = root2(vi);
+            const Two vi = fma2(mul2(two(s.beta2, s.beta2), two(v[i], v[i + 1])), one2, mul2(mul2(two(s.rest2, s.rest2), gi), gi));
+            apart(mi, m[i], m[i + 1]); apart(vi, v[i], v[i + 1]); apart(root2(vi), root[i], root[i + 1]);
+            top2 = max_nan(top2, root[i], root[i + 1]);
+        }
+        const bool beyond = !(top2 < INFINITE_ROOT);                         // a second moment that is infinite, or NaN
+        if (beyond) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) root[i] = v[i] == INFINITY ? INFINITY : root[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
             float a, b;
-            apart(fma2(ri, two(root_fix2, root_fix2), two(s.eps, s.eps)), a, b);
-            const Two wi = two(w[i], w[i + 1]), way = mul2(mul2(mi, two(fix1, fix1)), two(reciprocal_fast(a), reciprocal_fast(b)));
+            apart(fma2(two(root[i], root[i + 1]), two(root_fix2, root_fix2), two(s.eps, s.eps)), a, b);
+            const Two wi = two(w[i], w[i + 1]), way = mul2(mul2(two(m[i], m[i + 1]), two(fix1, fix1)), two(reciprocal_fast(a), reciprocal_fast(b)));
             apart(fma2(negative2(rate), fma2(two(decay, decay), wi, way), wi), w[i], w[i + 1]);
-            apart(mi, m[i], m[i + 1]); apart(vi, v[i], v[i + 1]); apart(ri, root[i], root[i + 1]);
         }
         if (view.master) store8(view.master, CUDARL_F32, at, wide, len, w);
         store8(view.param, view.param_type, at, wide, len, w);
@@ -436,10 +450,15 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
             store8(view.moment1, CUDARL_F32, at, wide, len, m);
             store8(view.moment2, CUDARL_F32, at, wide, len, v);
         } else {
-            // the largest magnitudes, in the order of their bits (values behind the tensor's end are zeros; NaN is the largest)
-            float top1 = 0.0f, top2 = 0.0f;
+            float top1 = 0.0f;                                               // (values behind the tensor's end are zeros; NaN is the largest)
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) { top1 = max_nan(top1, fabsf(m[i]), fabsf(m[i + 1])); top2 = max_nan(top2, root[i], root[i + 1]); }
+            for (int i = 0; i < 8; i += 2) top1 = max_nan(top1, fabsf(m[i]), fabsf(m[i + 1]));
+            if (beyond) {
+                top2 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { root[i] = root[i] == INFINITY ? INFINITE_ROOT : root[i]; top2 = max_nan(top2, root[i], root[i]); }
+            }
+            // the largest magnitudes of the block, in the order of their bits
             const float scale1 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top1))) * (1.0f / 448.0f), scale2 = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top2))) * (1.0f / 448.0f);
             if (lane == 0) { view.scale1[warp] = scale1; view.scale2[warp] = scale2; }
             float y1[8], y2[8], least = 448.0f;

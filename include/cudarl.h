@@ -277,6 +277,8 @@ int cudarl_policy_logprobs_backward(const cudarl_policy_rows* p, const float* st
  *   w' = w - lr lr_scale (weight_decay w + (m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps))
  * in 32 bits, rounded once to the weights' type (t = 1 for the first step).  With a master the step is that of the master and
  * `param` receives a copy rounded to its type.
+ * A v that passes a float's range is infinite: its value stays where it is from then on, but for the decay, until the moments
+ * are set anew (with 8 bits its root is kept as 2^65, and its block's scale goes by that).  Clipping keeps v from it.
  * With state_bits = 32 the moments m and v are floats.  With 8, moment1 holds m and moment2 the root of v as e4m3 codes, each
  * block of 256 consecutive values (the last may be shorter) times its scale: the block's largest magnitude / 448.  A code is
  * rounded up or down by 16 random bits of the Philox stream of (seed, step, place), so that small changes are not lost on

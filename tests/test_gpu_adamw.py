@@ -239,6 +239,87 @@ def test_large_and_small_gradients_in_one_block(pkg):
     assert ((t["param"] - w).abs() <= 0.02).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+@pytest.mark.parametrize("eps", [1e-30, 1e-8])
+@pytest.mark.parametrize("n", [256, 255])
+def test_gradients_over_a_floats_range(pkg, bits, grad, eps, n):
+    """A tensor of `n` values (loaded wide, and one by one) for every decade from 1e-20, where v is a few steps of the subnormal floats, to 1e38, where it is infinite
+    from 5.8e20 on; without clipping.  v is rounded by 2^-150 at the least, which is that much of its size and half as much of its root's; a root below 2^-50 is off by
+    2^-22 more."""
+    decades = list(range(-20, 39))
+    net = Net(pkg, [n] * len(decades), grad=grad, bits=bits, decay=0.01)
+    gen = torch.Generator("cuda").manual_seed(7)
+    for t, d in zip(net.tensors, decades):
+        for key in ("m", "v", "s1", "s2"):
+            if key in t:
+                t[key].zero_()
+        g = (0.7 + 0.3 * torch.rand(n, device="cuda", generator=gen, dtype=torch.float64)) * 10.0 ** d
+        t["grad"].copy_(g * (1 - 2 * torch.randint(0, 2, (n,), device="cuda", generator=gen)))
+    before = net.snapshot()
+    opt = pkg.AdamW(net.list(), state_bits=bits, eps=eps, seed=3)
+    opt.step(0.01)
+    eps, lr = float(np.float32(eps)), float(np.float32(0.01))
+    for i, (t, (w, g, m, v), d) in enumerate(zip(net.tensors, before, decades)):
+        lr_scale, decay = float(np.float32(1.0 + 0.5 * (i % 2))), float(np.float32(net.decay * (i % 3)))
+        em, ev = 0.1 * g, 0.001 * g * g
+        root = np.where(ev > plain.FLT_MAX, np.inf, np.sqrt(ev))
+        off = 0.5 * (5 * U + 2.0 ** -150 / ev) + 2.0 ** -22                  # of the root
+        step = lr * lr_scale * em / (1 - 0.9) / (root / np.sqrt(1 - 0.999) + eps)
+        ew = w - lr * lr_scale * decay * w - step
+        weight = t["param"].double().cpu().numpy()
+        assert np.isfinite(weight).all(), d
+        assert (np.abs(weight - ew) <= np.abs(step) * (24 * U + off) + 4 * U * np.abs(ew) + 4 * U * lr * decay * np.abs(w)).all(), d
+        if bits == 32:
+            got = t["v"].double().cpu().numpy()
+            if d > 20:
+                assert (got == np.inf).all()
+            else:
+                assert (np.abs(got - ev) <= 5 * U * ev + 2.0 ** -150).all()
+            assert (np.abs(t["m"].double().cpu().numpy() - em) <= 4 * U * np.abs(em)).all()
+        else:
+            _m, got = net.moments(t)
+            got = np.sqrt(got)
+            kept = np.where(np.isinf(root), 2.0 ** 65, root)
+            high = kept.max() / 448
+            assert abs(float(t["s2"][0]) - high) <= (2 * U + off.max()) * high
+            assert (np.abs(got - kept) <= kept * (2.0 ** -3 + off + 8 * U)).all()      # values within a factor of two of the block's largest: codes have three bits behind the first
+    for t in net.tensors:
+        t["grad"].zero_()
+    still = [t["param"].clone() for t in net.tensors]
+    opt.step(0.01)
+    for i, (t, w, d) in enumerate(zip(net.tensors, still, decades)):
+        assert torch.isfinite(t["param"]).all()
+        if d > 20:                                                           # stays where it is
+            w = w.double()
+            assert ((t["param"].double() - w * (1 - lr * (1.0 + 0.5 * (i % 2)) * net.decay * (i % 3))).abs() <= 2 * U * w.abs()).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_one_gradient_beyond_the_range(pkg, bits):
+    """Among ordinary ones: the others of its block take their step, nothing becomes NaN, zeros stay zeros."""
+    net = Net(pkg, [700], bits=bits)
+    t = net.tensors[0]
+    for key in ("m", "v", "s1", "s2"):
+        if key in t:
+            t[key].zero_()
+    t["grad"][5] = 3e30
+    t["grad"][6] = 0.0
+    before = net.snapshot()
+    opt = pkg.AdamW(net.list(), state_bits=bits)
+    opt.step(0.01)
+    (w, g, m, v), = before
+    ew, _m, _v = plain.adamw(w, g, m, v, 1, float(np.float32(0.01)), 0.0)
+    ew[5] = w[5]
+    got = t["param"].double().cpu().numpy()
+    assert (np.abs(got - ew) <= 40 * U * 0.01 + 2 * U * np.abs(ew)).all()
+    for _ in range(3):
+        opt.step(0.01)
+        assert torch.isfinite(t["param"]).all() and float(t["param"][5]) == float(w[5]) == got[5] and float(t["param"][6]) == float(w[6])
+        assert bits == 8 or torch.isfinite(t["m"]).all()
+        assert bits == 32 or (torch.isfinite(t["s1"]).all() and torch.isfinite(t["s2"]).all())
+
+
 def test_many_tensors_and_a_large_one(pkg):
     sizes = [int(n) for n in np.random.default_rng(3).integers(1, 3000, 900)] + [3_000_001]
     for bits in (32, 8):
