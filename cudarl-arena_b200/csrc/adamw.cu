@@ -664,21 +664,21 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
         s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;
     }
     if (s.clipped) {
-        k_grad_norm<<<o->norm_grid, 32 * WARPS, 0, st>>>(o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, o->norm_grid == o->pieces, grad_scale, c.max_grad_norm);
-        if ((e = cudaGetLastError()) != cudaSuccess) return fail_cuda("cudarl_adamw_step", e);
+        if ((e = launch(k_grad_norm, o->norm_grid, 32 * WARPS, st, o->dtensors, o->dpieces, o->pieces, o->dctl, o->dpart, o->norm_grid == o->pieces, grad_scale, c.max_grad_norm)) != cudaSuccess)
+            return fail_cuda("cudarl_adamw_step", e);
     }
-    cudaLaunchConfig_t launch = {};
-    launch.gridDim = dim3(o->grid); launch.blockDim = dim3(THREADS); launch.stream = st;
-    launch.dynamicSmemBytes = ring_bytes(c.state_bits);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(o->grid); cfg.blockDim = dim3(THREADS); cfg.stream = st;
+    cfg.dynamicSmemBytes = ring_bytes(c.state_bits);
     // after the norm's kernel: started while that one still runs, its first loads done, it waits for the norm on the device.  Without a norm it must not begin
     // before the gradients' own kernel has ended
     cudaLaunchAttribute early[1];
     early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; early[0].val.programmaticStreamSerializationAllowed = 1;
-    if (s.clipped) { launch.attrs = early; launch.numAttrs = 1; }
+    if (s.clipped) { cfg.attrs = early; cfg.numAttrs = 1; }
     const Tensor* tensors = o->dtensors;
     const Piece* pieces = o->dpieces;
-    e = c.state_bits == 32 ? cudaLaunchKernelEx(&launch, k_adamw<32>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale)
-                           : cudaLaunchKernelEx(&launch, k_adamw<8>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale);
+    e = c.state_bits == 32 ? cudaLaunchKernelEx(&cfg, k_adamw<32>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale)
+                           : cudaLaunchKernelEx(&cfg, k_adamw<8>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale);
     return e == cudaSuccess ? 0 : fail_cuda("cudarl_adamw_step", e);
 }
 

@@ -9,10 +9,20 @@
 
 namespace cudarl {
 
+// A call of the runtime that fails is remembered by it until somebody asks.  What has been reported here is forgotten there, so that no later call takes it for its own.
 inline int fail_cuda(const char* what, cudaError_t e) noexcept {
+    cudaGetLastError();
     char text[256];
     std::snprintf(text, sizeof text, "%s: %s", what, cudaGetErrorString(e));
     return fail_global(1000 + (int)e, text);
+}
+
+// A launch that answers for itself (cudaGetLastError after a launch would also give what an earlier call has left).
+template <class... Params, class... Args>
+inline cudaError_t launch(void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(block); cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 inline size_t type_bytes(int type) { return type == CUDARL_F32 ? 4u : 2u; }
@@ -32,7 +42,7 @@ public:
         }
         cudaPointerAttributes a;
         const cudaError_t e = cudaPointerGetAttributes(&a, p);
-        if (e != cudaSuccess) { cudaGetLastError(); return fail_cuda("cudaPointerGetAttributes", e); }
+        if (e != cudaSuccess) return fail_cuda("cudaPointerGetAttributes", e);
         if (a.type == cudaMemoryTypeManaged) return 0;
         if (a.type != cudaMemoryTypeDevice) {
             std::snprintf(text, sizeof text, "%s is not device memory", name);

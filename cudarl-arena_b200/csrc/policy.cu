@@ -1110,15 +1110,12 @@ constexpr int SHORT_ACTIONS = 128, WARP_ACTIONS = 1024;
 template <int TYPE, int G, int E, bool WIDE>
 cudaError_t launch_short(const Rows& p, const Outputs& o, cudaStream_t st) {
     const unsigned grid = blocks_of(p.rows, 256 / G);
-    if (o.top) k_short<TYPE, G, E, WIDE, true><<<grid, 256, 0, st>>>(p, o);
-    else k_short<TYPE, G, E, WIDE, false><<<grid, 256, 0, st>>>(p, o);
-    return cudaGetLastError();
+    return o.top ? launch(k_short<TYPE, G, E, WIDE, true>, grid, 256, st, p, o) : launch(k_short<TYPE, G, E, WIDE, false>, grid, 256, st, p, o);
 }
 struct BackwardArgs { const float4* stats; const float* gl; const float* gh; void* grad; long long stride; };
 template <int TYPE, int G, int E, bool WIDE>
 cudaError_t launch_short(const Rows& p, const BackwardArgs& b, cudaStream_t st) {
-    k_short_backward<TYPE, G, E, WIDE><<<blocks_of(p.rows, 256 / G * (G == 1 && E == 4 ? 2 : 1)), 256, 0, st>>>(p, b.gl, b.gh, b.grad, b.stride);
-    return cudaGetLastError();
+    return launch(k_short_backward<TYPE, G, E, WIDE>, blocks_of(p.rows, 256 / G * (G == 1 && E == 4 ? 2 : 1)), 256, st, p, b.gl, b.gh, b.grad, b.stride);
 }
 // Rows of up to SHORT_ACTIONS actions, either way (a call's outputs or a gradient's arguments).
 template <int TYPE, class Args>
@@ -1141,22 +1138,14 @@ cudaError_t launch_warp(const Rows& p, const Outputs& o, int sms, cudaStream_t s
     while (group < 32 && group * 2 * (o.top ? o.top : 1) <= GROUP_KEYS && p.rows >= 16ll * group * most) group *= 2;
     const bool alike = p.stride * (long long)sizeof(typename Of<TYPE>::T) % 16 == 0;
     const unsigned all = blocks_of(p.rows, 8 * group), grid = all < most ? all : most;
-    if (p.legal) {
-        if (o.top) k_warp<TYPE, CHUNKS, true, true><<<grid, 256, 0, st>>>(p, o, group, alike);
-        else k_warp<TYPE, CHUNKS, true, false><<<grid, 256, 0, st>>>(p, o, group, alike);
-    } else {
-        if (o.top) k_warp<TYPE, CHUNKS, false, true><<<grid, 256, 0, st>>>(p, o, group, alike);
-        else k_warp<TYPE, CHUNKS, false, false><<<grid, 256, 0, st>>>(p, o, group, alike);
-    }
-    return cudaGetLastError();
+    if (p.legal) return o.top ? launch(k_warp<TYPE, CHUNKS, true, true>, grid, 256, st, p, o, group, alike) : launch(k_warp<TYPE, CHUNKS, true, false>, grid, 256, st, p, o, group, alike);
+    return o.top ? launch(k_warp<TYPE, CHUNKS, false, true>, grid, 256, st, p, o, group, alike) : launch(k_warp<TYPE, CHUNKS, false, false>, grid, 256, st, p, o, group, alike);
 }
 template <int TYPE, int VALUES>
 cudaError_t launch_warp(const Rows& p, const BackwardArgs& b, int sms, cudaStream_t st) {
     constexpr int CHUNKS = VALUES / 32 / Chunk<TYPE>::N;
     const unsigned most = (unsigned)(sms * warp_blocks(VALUES / 32)), all = blocks_of(p.rows, 8), grid = all < most ? all : most;
-    if (p.legal) k_warp_backward<TYPE, CHUNKS, true><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
-    else k_warp_backward<TYPE, CHUNKS, false><<<grid, 256, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
-    return cudaGetLastError();
+    return launch(p.legal ? k_warp_backward<TYPE, CHUNKS, true> : k_warp_backward<TYPE, CHUNKS, false>, grid, 256, st, p, b.stats, b.gl, b.gh, b.grad, b.stride);
 }
 
 template <int TYPE, int T, bool MASKED, bool TOP>
@@ -1215,10 +1204,9 @@ cudaError_t launch_backward(const Rows& p, const BackwardArgs& b, int sms, cudaS
     // 67 / 43 us, 40000 x 1500 bf16 113 / 50; at most 256 / 128: 20000 x 6000 bf16 86 / 82, 10000 x 9000 masked 105 / 86, 20000 x 2500 fp32 63.5 / 67.6)
     const int chunks = v / Chunk<TYPE>::N, most = PIECE_THREADS * UNROLL, pieces = (chunks + most - 1) / most, each = (chunks + pieces * UNROLL - 1) / (pieces * UNROLL);
     const int threads = each <= 64 ? 64 : (each + 31) / 32 * 32;
-    const dim3 grid((unsigned)pieces, (unsigned)(p.rows < 65535 ? p.rows : 65535));
-    if (p.legal) k_long_backward<TYPE, true><<<grid, threads, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
-    else k_long_backward<TYPE, false><<<grid, threads, 0, st>>>(p, b.stats, b.gl, b.gh, b.grad, b.stride);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)pieces, (unsigned)(p.rows < 65535 ? p.rows : 65535)); cfg.blockDim = dim3((unsigned)threads); cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, p.legal ? k_long_backward<TYPE, true> : k_long_backward<TYPE, false>, p, b.stats, b.gl, b.gh, b.grad, b.stride);
 }
 
 }  // namespace

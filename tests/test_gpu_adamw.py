@@ -504,3 +504,41 @@ def test_a_policy_steps_the_arena_and_learns(pkg, bits):
     s = opt.get_stats()
     want = torch.cat([k.reshape(-1) for k in keep]).double().norm()
     assert abs(s.grad_norm - float(want)) <= 1e-9 * float(want)
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+def test_calls_after_a_refused_one(pkg, max_norm):
+    """What failed and was reported -- an optimizer or a world on a device that is not there -- is not reported again by the next call, whose kernels it has nothing to do with."""
+    net = Net(pkg, [3000, 50])
+    opt = pkg.AdamW(net.list(), max_grad_norm=max_norm)
+    nowhere = pkg.make_config(4, 4, 2, 1)
+    nowhere.device = 1000
+    x, lp, grad = (torch.randn(6, v, device="cuda") for v in (1500, 1, 1500))
+    taken = torch.zeros(6, dtype=torch.int32, device="cuda")
+    stats = torch.zeros(6, 4, device="cuda")
+
+    def refused(first):
+        if first:
+            with pytest.raises(pkg.CudarlError):
+                pkg.AdamW(net.list(), device=1000)
+        else:
+            with pytest.raises(pkg.CudarlError):
+                pkg.VecGridWorld(nowhere)
+
+    world = pkg.VecGridWorld(pkg.make_config(4, 4, 2, 1))
+    for first in (True, False):
+        before = net.snapshot()
+        step = int(opt.get_stats().step) + 1
+        refused(first)
+        opt.step(0.01)
+        norm = np.sqrt(sum((g ** 2).sum() for _w, g, _m, _v in before))
+        check(net, before, step, 0.01, min(1.0, max_norm / (norm + 1e-6)) if max_norm else 1.0)
+        for v in (7, 300, 1500):
+            rows = pkg.PolicyRows(x.data_ptr(), pkg.F32, 6, v, row_stride=1500, taken=taken.data_ptr())
+            refused(first)
+            pkg.policy_logprobs(rows, lp.data_ptr(), stats=stats.data_ptr())
+            refused(first)
+            pkg.policy_logprobs_backward(rows, stats.data_ptr(), lp.data_ptr(), None, grad.data_ptr(), 1500)
+    refused(True)
+    world.train_steps(2)                                                     # the arena's own calls neither
+    world.synchronize()
