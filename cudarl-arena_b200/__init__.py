@@ -140,6 +140,7 @@ ABI = {
     "cudarl_adamw_step": (C.c_int, [_P, C.c_float, C.c_float, _P]),
     "cudarl_adamw_set_gradients": (C.c_int, [_P, C.POINTER(_P), _P]),
     "cudarl_adamw_get_stats": (C.c_int, [_P, C.POINTER(AdamWStats)]),
+    "cudarl_debug_adamw_set_copy_wait_polls": (C.c_int, [_P, C.c_int32]),
     "cudarl_version": (C.c_char_p, []),
 }
 
@@ -469,3 +470,6 @@ class AdamW:
         s = AdamWStats()
         _global_ck(self.lib.cudarl_adamw_get_stats(self.h, C.byref(s)))
         return s
+
+    def debug_set_copy_wait_polls(self, polls):
+        _global_ck(self.lib.cudarl_debug_adamw_set_copy_wait_polls(self.h, polls))

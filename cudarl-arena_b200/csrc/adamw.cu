@@ -39,7 +39,7 @@ struct Piece { unsigned tensor, block, blocks, number; };   // `blocks` blocks (
 struct Control {
     long long step, skipped;
     double norm, power1, power2;              // powers of the betas for the step to come ...
-    float fix1, root_fix2;                    // ... and what they make of it: 1 / (1 - power1), and the root of 1 / (1 - power2)
+    float fix1, root_fix2;                    // ... and what they make of it: 1 / (1 - power1), and the root of 1 / (1 - power2).  fix1 is 0 once a wait has run out
     float clip;
     unsigned go;                              // 0: the norm was no finite number
     unsigned done, done_norm;                 // blocks of the launch that have finished
@@ -51,6 +51,7 @@ struct Settings {
     float one;                                // 1
     unsigned keys[20];                        // of the ten Philox rounds
     int clipped;
+    unsigned polls;                           // > 0: of a test, see cudarl_debug_adamw_set_copy_wait_polls
     double power1, power2;                    // the betas
 };
 
@@ -134,13 +135,17 @@ __device__ __forceinline__ void from_codes(unsigned v, float* x) {           // 
     }
 }
 
-__device__ __forceinline__ bool last_block(unsigned* done) {
-    __syncthreads();
+// Whether this is thread 0 of the launch's last block, and whether any warp of any block has given up a wait: those blocks count in the upper half, too (no more
+// than three blocks an SM: the lower half does not run over).
+__device__ __forceinline__ bool last_block(unsigned* done, bool gave_up, bool& broken) {
+    broken = __syncthreads_or(gave_up);
     if (threadIdx.x != 0u) return false;
     __threadfence();
-    if (atomicAdd(done, 1u) + 1u != gridDim.x) return false;
+    const unsigned before = atomicAdd(done, broken ? 0x10001u : 1u);
+    if ((before & 0xFFFFu) + 1u != gridDim.x) return false;
     __threadfence();
     *done = 0u;
+    broken = broken || before >> 16;
     return true;
 }
 
@@ -176,9 +181,11 @@ template <int BITS> __device__ void init_ring(Ring<BITS>& ring) {
 }
 
 // The copying warp (a call of its own: its registers are not the computing warps').  Its lanes look up 32 pieces at a time, then each has its own copied when its turn and a stage come.
-template <int BITS> __device__ __noinline__ void copy_pieces(Ring<BITS>& ring, const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl) {
+// Whoever gives up a wait, this warp returns when what it has begun has landed (or a wait for that has run out, too): until then the block does not end.
+template <int BITS> __device__ __noinline__ bool copy_pieces(Ring<BITS>& ring, const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl) {
     const unsigned lane = threadIdx.x % 32u;
-    unsigned at = 0u, parity = 1u;                                           // the stage that is next, and which phase of `empty` lets it be filled
+    constexpr unsigned STAGES = Ring<BITS>::STAGES;
+    unsigned at = 0u, parity = 1u, begun = 0u;                               // the stage that is next, which phase of `empty` lets it be filled, and pieces so far
     bool fine = true;
     for (unsigned long long base = blockIdx.x; base < n && fine; base += 32ull * gridDim.x) {
         const unsigned long long k = base + (unsigned long long)lane * gridDim.x;
@@ -200,6 +207,8 @@ template <int BITS> __device__ __noinline__ void copy_pieces(Ring<BITS>& ring, c
         for (unsigned turn = 0; turn < 32u && base + (unsigned long long)turn * gridDim.x < n && fine; ++turn) {
             Stage<BITS>& st = ring.stage[at];
             unsigned long long* const bar = &ring.full[at];
+            // from here on it waits for the computing warps, and they for the norm: how long that takes is not this wait's
+            if (begun == STAGES) asm volatile("griddepcontrol.wait;" ::: "memory");
             if (lane == turn) fine = mbar_wait(&ring.empty[at], parity, 0u);
             fine = __shfl_sync(~0u, fine, turn);
             if (!fine) break;
@@ -222,17 +231,14 @@ template <int BITS> __device__ __noinline__ void copy_pieces(Ring<BITS>& ring, c
                 }
             }
             __syncwarp();
-            if (++at == Ring<BITS>::STAGES) { at = 0u; parity ^= 1u; }
+            ++begun;
+            if (++at == STAGES) { at = 0u; parity ^= 1u; }
         }
     }
-    if (!fine) {                                                             // given up: nothing may still be under way when the block ends
-        if (lane == 0u) {
-            atomicOr(&ctl->error, ERR_COPY_TIMEOUT);
-            for (int i = 0; i < Ring<BITS>::STAGES; ++i) { (void)mbar_wait(&ring.full[i], 0u, 1u << 16); (void)mbar_wait(&ring.full[i], 1u, 1u << 16); }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncwarp();
-    }
+    for (unsigned i = 0; i < STAGES && i < begun; ++i)                       // the last phase that each stage was begun for
+        fine = __all_sync(~0u, mbar_wait(&ring.full[i], ((begun - 1u - i) / STAGES) & 1u, 0u)) && fine;
+    if (!fine && lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT);
+    return fine;
 }
 
 // Eight values of a block in a stage: 32 or 16 bytes a lane.
@@ -373,11 +379,16 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
     init_ring(ring);
     const unsigned lane = threadIdx.x % 32u, warp = threadIdx.x / 32u;
     const bool copies = warp == WARPS;
-    if (copies) copy_pieces(ring, tensors, pieces, n, ctl);                  // (what it copies is not what the norm's kernel writes)
+    bool gave_up = false;
+    if (s.polls) {                                                           // there are no pieces then: a wait for copies that nobody begins
+        gave_up = !__all_sync(~0u, mbar_wait(&ring.full[0], 0u, s.polls));
+        if (gave_up && lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT);
+    }
+    if (copies) gave_up = !copy_pieces(ring, tensors, pieces, n, ctl) || gave_up;      // (what it copies is not what the norm's kernel writes)
     asm volatile("griddepcontrol.wait;" ::: "memory");                       // for the norm, when there is one
     const long long step = __ldcg(&ctl->step);
     const float fix1 = __ldcg(&ctl->fix1), root_fix2 = __ldcg(&ctl->root_fix2);
-    const bool go = !s.clipped || __ldcg(&ctl->go);
+    const bool go = fix1 != 0.0f && (!s.clipped || __ldcg(&ctl->go));        // once a wait has run out, no step does anything
     const float scale = s.clipped ? grad_scale * __ldcg(&ctl->clip) : grad_scale;
     unsigned prefix[4];
     policy_prefix(s.keys, (unsigned long long)(step + 1), prefix);
@@ -385,7 +396,11 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
     for (unsigned long long k = blockIdx.x; k < n && !copies; k += gridDim.x) {
         Stage<BITS>& st = ring.stage[place];
         unsigned long long* const empty = &ring.empty[place];
-        if (!mbar_wait(&ring.full[place], parity, 0u)) { if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT); break; }
+        if (!__all_sync(~0u, mbar_wait(&ring.full[place], parity, 0u))) {    // (what is under way the copying warp waits for)
+            gave_up = true;
+            if (lane == 0u) atomicOr(&ctl->error, ERR_COPY_TIMEOUT);
+            break;
+        }
         if (++place == Ring<BITS>::STAGES) { place = 0u; parity ^= 1u; }
         const View& view = st.view;
         if (warp < view.blocks && go) {
@@ -508,12 +523,14 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tenso
         __syncwarp();
         if (lane == 0u) mbar_arrive(empty);                                  // the stage can be filled again
     }
-    if (last_block(&ctl->done)) {
-        if (go) {
+    bool broken;
+    if (last_block(&ctl->done, gave_up, broken)) {
+        if (broken) ctl->fix1 = 0.0f;                                        // a step that was broken off does not count, and is the last
+        else if (go) {
             const double p1 = ctl->power1 * s.power1, p2 = ctl->power2 * s.power2;
             ctl->step = step + 1; ctl->power1 = p1; ctl->power2 = p2;
             ctl->fix1 = (float)(1.0 / (1.0 - p1)); ctl->root_fix2 = (float)sqrt(1.0 / (1.0 - p2));
-        } else ctl->skipped += 1;
+        } else if (fix1 != 0.0f) ctl->skipped += 1;
     }
 }
 
@@ -528,6 +545,7 @@ struct cudarl_adamw {
     double* dpart = nullptr;
     unsigned pieces = 0, grid = 0, norm_grid = 0;
     bool gradients = false;                  // every tensor with values has one
+    unsigned polls = 0;
 };
 
 namespace {
@@ -658,7 +676,7 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
     if (e != cudaSuccess) return fail_cuda("cudaSetDevice", e);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudarl_adamw_config& c = o->cfg;
-    Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, 1.0f, {}, c.max_grad_norm > 0.0f, c.beta1, c.beta2};
+    Settings s{(float)c.beta1, (float)(1.0 - c.beta1), (float)c.beta2, (float)(1.0 - c.beta2), (float)c.eps, 1.0f, {}, c.max_grad_norm > 0.0f, o->polls, c.beta1, c.beta2};
     for (unsigned r = 0; r < 10; ++r) {
         s.keys[2 * r] = (unsigned)c.seed + r * 0x9E3779B9u;
         s.keys[2 * r + 1] = ((unsigned)(c.seed >> 32) ^ TAG_OPTIMIZER) + r * 0xBB67AE85u;
@@ -677,8 +695,9 @@ extern "C" int cudarl_adamw_step(cudarl_adamw* o, float lr, float grad_scale, vo
     if (s.clipped) { cfg.attrs = early; cfg.numAttrs = 1; }
     const Tensor* tensors = o->dtensors;
     const Piece* pieces = o->dpieces;
-    e = c.state_bits == 32 ? cudaLaunchKernelEx(&cfg, k_adamw<32>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale)
-                           : cudaLaunchKernelEx(&cfg, k_adamw<8>, tensors, pieces, o->pieces, o->dctl, s, lr, grad_scale);
+    const unsigned n = o->polls ? 0u : o->pieces;
+    e = c.state_bits == 32 ? cudaLaunchKernelEx(&cfg, k_adamw<32>, tensors, pieces, n, o->dctl, s, lr, grad_scale)
+                           : cudaLaunchKernelEx(&cfg, k_adamw<8>, tensors, pieces, n, o->dctl, s, lr, grad_scale);
     return e == cudaSuccess ? 0 : fail_cuda("cudarl_adamw_step", e);
 }
 
@@ -718,5 +737,12 @@ extern "C" int cudarl_adamw_get_stats(cudarl_adamw* o, cudarl_adamw_stats* out) 
     if ((e = cudaDeviceSynchronize()) != cudaSuccess || (e = cudaMemcpy(&c, o->dctl, sizeof c, cudaMemcpyDeviceToHost)) != cudaSuccess) return fail_cuda("cudarl_adamw_get_stats", e);
     out->step = c.step; out->skipped = c.skipped; out->grad_norm = c.norm;
     if (c.error) return fail_global(CUDARL_ERR_DEVICE + (int)c.error, "a wait of the optimizer's kernel ran out: its tensors are not to be used");
+    return 0;
+}
+
+extern "C" int cudarl_debug_adamw_set_copy_wait_polls(cudarl_adamw* o, int32_t polls) {
+    if (!o) return fail_global(-1, "null argument");
+    if (polls < 0) return fail_global(-1, "polls negative");
+    o->polls = (unsigned)polls;
     return 0;
 }

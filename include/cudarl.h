@@ -326,8 +326,12 @@ void cudarl_adamw_destroy(cudarl_adamw* opt);
 int  cudarl_adamw_step(cudarl_adamw* opt, float lr, float grad_scale, void* stream);
 /* New gradient pointers for the tensors in order (host array of `count` device pointers); not while `stream` is captured. */
 int  cudarl_adamw_set_gradients(cudarl_adamw* opt, const void* const* grads, void* stream);
-/* Waits for the device. */
+/* Waits for the device.  CUDARL_ERR_DEVICE + CUDARL_DEVERR_COPY_TIMEOUT (statistics filled in) when a wait inside a step ran out: that
+ * step is not counted, a part of the tensors may have taken it, and no later step of the handle does anything. */
 int  cudarl_adamw_get_stats(cudarl_adamw* opt, cudarl_adamw_stats* out);
+/* For tests, as cudarl_debug_set_copy_wait_polls: with polls > 0 the steps launched from now on first wait for copies that nobody has begun, for that many
+ * tries, and give up.  0 = the usual limit of two seconds for each wait. */
+int  cudarl_debug_adamw_set_copy_wait_polls(cudarl_adamw* opt, int32_t polls);
 
 /* Switch the max(0, .) clamp of the flat reference kernel (src/kernels.cu:102-110) on or off. */
 int cudarl_set_legacy_clamp(cudarl_ctx* ctx, int on);

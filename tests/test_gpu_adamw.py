@@ -542,3 +542,32 @@ def test_calls_after_a_refused_one(pkg, max_norm):
     refused(True)
     world.train_steps(2)                                                     # the arena's own calls neither
     world.synchronize()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+def test_a_wait_that_runs_out(pkg, bits, max_norm):
+    """The step gives up (its wait is for copies that nobody has begun), is not counted and is reported; no later step of the handle does anything; the GPU and a new
+    handle go on."""
+    net = Net(pkg, [300, 50000, 7], "bf16", "bf16", True, bits)
+    opt = pkg.AdamW(net.list(), state_bits=bits, max_grad_norm=max_norm, step=4)
+    opt.step(0.01)
+    whole = [a.clone() for a, _o, _n in net.all]
+    opt.debug_set_copy_wait_polls(3)
+    opt.step(0.01)
+    stats = pkg.AdamWStats()
+    for _ in range(2):
+        assert pkg.load().cudarl_adamw_get_stats(opt.h, C.byref(stats)) == 3000 + 32 and (stats.step, stats.skipped) == (5, 0)
+        opt.debug_set_copy_wait_polls(0)
+        opt.step(0.01)                                                       # launched as usual, and leaves everything as it is
+    with pytest.raises(pkg.CudarlError, match="ran out"):
+        opt.get_stats()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, (b, _o, _n) in zip(whole, net.all))
+    before = net.snapshot()
+    norm = np.sqrt(sum((g ** 2).sum() for _w, g, _m, _v in before))
+    opt = pkg.AdamW(net.list(), state_bits=bits, max_grad_norm=max_norm, step=5)
+    opt.step(0.01)
+    check(net, before, 6, 0.01, min(1.0, max_norm / (norm + 1e-6)) if max_norm else 1.0)
+    assert opt.get_stats().step == 6
+    with pytest.raises(pkg.CudarlError, match="polls"):
+        opt.debug_set_copy_wait_polls(-1)

@@ -82,3 +82,7 @@ def test_null_arguments_are_refused(pkg):
     assert lib.cudarl_adamw_set_gradients(None, None, None) == -1
     assert lib.cudarl_adamw_get_stats(None, C.byref(s)) == -1
     lib.cudarl_adamw_destroy(None)
+
+
+def test_the_debug_call_is_refused(pkg):
+    assert pkg.load().cudarl_debug_adamw_set_copy_wait_polls(None, 1) == -1 and "null" in text(pkg)
