@@ -29,6 +29,7 @@ EPS_FIXED, EPS_MULT_PER_STEP, EPS_MULT_PER_EPISODE, EPS_LINEAR = 0, 1, 2, 3
 QINIT_ZERO, QINIT_UNIFORM = 0, 1
 F32, BF16, F16 = 0, 1, 2
 MAX_TOP = 32
+ACTIONS_WITHOUT_STATS = 128
 ADAMW_BLOCK = 256
 
 
@@ -429,7 +430,10 @@ def policy_logprobs(rows, logprob=None, entropy=None, stats=None, top=0, top_act
 
 
 def policy_logprobs_backward(rows, stats, grad_logprob, grad_entropy, grad_logits, grad_stride=None, stream=None):
-    """cudarl_policy_logprobs_backward: the gradient of the logits, with the `stats` that policy_logprobs wrote for the same rows."""
+    """cudarl_policy_logprobs_backward: the gradient of the logits, with the `stats` that policy_logprobs wrote for the same rows (rows of up to
+    ACTIONS_WITHOUT_STATS actions need none: None)."""
+    if stats is None and rows.actions <= ACTIONS_WITHOUT_STATS:
+        stats = grad_logits                                   # an address; it is not looked at
     rc = load().cudarl_policy_logprobs_backward(rows, stats, grad_logprob, grad_entropy, grad_logits, rows.actions if grad_stride is None else grad_stride, stream)
     if rc != 0:
         _global_ck(rc)

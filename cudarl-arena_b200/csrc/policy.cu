@@ -1105,7 +1105,7 @@ bool aligned_rows(const void* base, long long stride, int value, int bytes) {
     return reinterpret_cast<uintptr_t>(base) % (unsigned)bytes == 0 && stride * value % bytes == 0;
 }
 
-constexpr int SHORT_ACTIONS = 128, WARP_ACTIONS = 1024;
+constexpr int SHORT_ACTIONS = CUDARL_ACTIONS_WITHOUT_STATS, WARP_ACTIONS = 1024;
 
 template <int TYPE, int G, int E, bool WIDE>
 cudaError_t launch_short(const Rows& p, const Outputs& o, cudaStream_t st) {
@@ -1248,7 +1248,7 @@ extern "C" int cudarl_policy_logprobs_backward(const cudarl_policy_rows* p, cons
     CallerArrays arrays;
     const size_t align = type_bytes(p->type);
     if ((rc = arrays.check("logits", p->logits, align)) || (rc = arrays.check_if("legal", p->legal, 1)) || (rc = arrays.check_if("taken", p->taken, 4)) ||
-        (rc = arrays.check("stats", stats, 16)) || (rc = arrays.check_if("grad_logprob", grad_logprob, 4)) || (rc = arrays.check_if("grad_entropy", grad_entropy, 4)) ||
+        (p->actions > SHORT_ACTIONS && (rc = arrays.check("stats", stats, 16))) || (rc = arrays.check_if("grad_logprob", grad_logprob, 4)) || (rc = arrays.check_if("grad_entropy", grad_entropy, 4)) ||
         (rc = arrays.check("grad_logits", grad_logits, align))) return rc;
     CurrentDevice current;
     int sms = 0;

@@ -235,6 +235,7 @@ int cudarl_get_traps(cudarl_ctx* ctx, int32_t capacity, int32_t* cells, float* p
 enum { CUDARL_F32 = 0, CUDARL_BF16 = 1, CUDARL_F16 = 2 };
 #define CUDARL_MAX_TOP 32
 #define CUDARL_MAX_POLICY_ACTIONS (1 << 30)
+#define CUDARL_ACTIONS_WITHOUT_STATS 128
 
 /* Rows of logits.  Row r, action a is logits[r*row_stride + a], of the type given, at any alignment that the type has; the log
  * probabilities are those of the distribution softmax(inv_temperature * logits) over the legal actions.  An action whose mask
@@ -255,7 +256,8 @@ typedef struct cudarl_policy_rows {
 } cudarl_policy_rows;
 
 /* logprob[rows]: of the action taken.  entropy[rows]: in nats.  stats[4*rows], 16-byte aligned: what the backward call reads (rows of up to
- * 128 actions need none: it is left as it is).
+ * CUDARL_ACTIONS_WITHOUT_STATS actions need none: it is left as it is, and the backward call does not look at what it is given for it -- any address but
+ * NULL will do).
  * top_actions / top_logprobs [rows*top]: the `top` (0 .. CUDARL_MAX_TOP) most probable actions in falling order, of equal
  * logits the lowest action first; places that no action is left for hold -1 and minus infinity.  Any output may be NULL (the
  * two top arrays only together with top = 0).

@@ -398,3 +398,26 @@ def test_gradient_against_differences(pkg):
         d = (loss(up) - loss(down)) / (up[:, j].astype(np.float64) - down[:, j].astype(np.float64))
         # third derivatives of log p and H are at most 1 and 6 + 2 H (H <= log 11); outputs are off by 2^-16 at most
         assert (np.abs(d - g[:, j]) <= (np.abs(gl) + 11 * np.abs(gh)) * (step ** 2 / 6 + 2.0 ** -16 / step)).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [1, 4, 33, 127, 128, 129])
+def test_gradients_of_short_rows_without_statistics(pkg, t, v):
+    """Up to 128 actions: neither written nor read, so that None, or any address, gives the same gradient; from 129 on they are needed."""
+    n = 37
+    x, taken = torch.randn(n, v, device="cuda").to(TYPES[t]), torch.randint(0, v, (n,), device="cuda", dtype=torch.int32)
+    gl, gh = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+    p, out, _keep = forward(pkg, x, t, taken, stats=True)
+    grads = [torch.full_like(x, 77) for _ in range(3)]
+    pkg.policy_logprobs_backward(p, out[4].data_ptr(), gl.data_ptr(), gh.data_ptr(), grads[0].data_ptr())
+    torch.cuda.synchronize()
+    if v > pkg.ACTIONS_WITHOUT_STATS:
+        with pytest.raises(pkg.CudarlError, match="stats"):
+            pkg.policy_logprobs_backward(p, None, gl.data_ptr(), gh.data_ptr(), grads[1].data_ptr())
+        with pytest.raises(pkg.CudarlError, match="stats is not aligned"):
+            pkg.policy_logprobs_backward(p, out[4].data_ptr() + 4, gl.data_ptr(), gh.data_ptr(), grads[1].data_ptr())
+        return
+    assert (out[4] == 77).all()
+    pkg.policy_logprobs_backward(p, None, gl.data_ptr(), gh.data_ptr(), grads[1].data_ptr())
+    pkg.policy_logprobs_backward(p, 4, gl.data_ptr(), gh.data_ptr(), grads[2].data_ptr())
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])

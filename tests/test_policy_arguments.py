@@ -86,3 +86,12 @@ def test_null_arguments_are_refused(pkg):
 
 def test_the_debug_call_is_refused(pkg):
     assert pkg.load().cudarl_debug_adamw_set_copy_wait_polls(None, 1) == -1 and "null" in text(pkg)
+
+
+def test_short_rows_need_no_statistics(pkg):
+    """The gradient of rows of up to 128 actions takes the sums anew: there None is fine (what is refused here is the address of the logits), above not."""
+    assert pkg.ACTIONS_WITHOUT_STATS == 128
+    for actions, word in ((1, None), (128, None), (129, "stats"), (5000, "stats")):
+        with pytest.raises(pkg.CudarlError) as e:
+            pkg.policy_logprobs_backward(rows(pkg, actions=actions), None, A, A, A)
+        assert ("stats" in str(e.value)) == (word is not None)
