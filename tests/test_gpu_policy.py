@@ -421,3 +421,94 @@ def test_gradients_of_short_rows_without_statistics(pkg, t, v):
     pkg.policy_logprobs_backward(p, None, gl.data_ptr(), gh.data_ptr(), grads[1].data_ptr())
     pkg.policy_logprobs_backward(p, 4, gl.data_ptr(), gh.data_ptr(), grads[2].data_ptr())
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+# rows and actions for every way to split the work: single lanes, teams, a warp, 128 threads, clusters of 2, 4 and 8 blocks (which of them goes by the type, too)
+SPLITS = [(1500, 4), (1500, 100), (1500, 257), (3000, 700), (1300, 2500), (1200, 8191), (400, 5003), (400, 9001), (300, 33001), (140, 20001), (70, 40003), (7, 70001), (2, 131075)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("n,v", SPLITS)
+def test_one_value_in_every_chunk(pkg, t, masked, top, n, v):
+    """A row that holds one value -- all others are minus infinity, or masked -- which is in turn at either end and in every chunk of 16 bytes, in rows at every alignment:
+    a value that is left out leaves nothing, one that counts twice halves the probability; in the gradient every place is written once."""
+    rng = np.random.default_rng(v)
+    per = 4 if t == "f32" else 8
+    places = np.concatenate([np.arange(min(v, 40)), np.arange(max(0, v - 40), v), np.arange(0, v - per, per) + np.arange(len(range(0, v - per, per))) % per]) if v > 1100 else np.arange(v)
+    places = np.concatenate([places, rng.integers(0, v, -len(places) % n)])
+    stride = v + 1
+    buffer = torch.full((3 + n * stride,), 0.5 if masked else -np.inf, dtype=TYPES[t], device="cuda")
+    view = torch.as_strided(buffer, (n, v), (stride, 1), 3)
+    legal = torch.zeros(n, v + 1, dtype=torch.uint8, device="cuda")[:, :v] if masked else None
+    gl, one = torch.ones(n, device="cuda"), torch.ones(n, 1, device="cuda")
+    grad = torch.empty(n, v, dtype=TYPES[t], device="cuda")
+    fails = torch.zeros((), dtype=torch.int64, device="cuda")
+    for at in range(0, len(places), n):
+        j = torch.from_numpy(places[at:at + n].astype(np.int32)).cuda()
+        jl = j.long()[:, None]
+        if masked:
+            legal.scatter_(1, jl, 1)
+        else:
+            view.scatter_(1, jl, 0.5)
+        _p, (lp, h, ta, tl, _st), _keep = forward(pkg, view, t, j, legal, top=top)
+        fails += (~(lp[:n].abs() <= 1e-6)).sum() + (~(h[:n].abs() <= 1e-6)).sum()
+        if top:
+            fails += (ta[:n * top].view(n, top)[:, 0] != j).sum() + (ta[:n * top].view(n, top)[:, 1:] != -1).sum() + (~(tl[:n * top].view(n, top)[:, 0].abs() <= 1e-6)).sum()
+        else:
+            other = (j + 1 + v // 3) % v                                     # the action taken is one without any probability: 1 there, -1 where the value is
+            p, (_lp, _h, _ta, _tl, st), _keep = forward(pkg, view, t, other, legal, stats=True)
+            grad.fill_(77)
+            pkg.policy_logprobs_backward(p, st.data_ptr(), gl.data_ptr(), None, grad.data_ptr())
+            g = grad.float()
+            g.scatter_add_(1, jl, one)
+            if not masked:
+                g.scatter_add_(1, other.long()[:, None], -one)
+            fails += (~(g.abs() <= 1e-6)).sum()
+        if masked:
+            legal.scatter_(1, jl, 0)
+        else:
+            view.scatter_(1, jl, -np.inf)
+    assert int(fails) == 0
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n,v", [s for s in SPLITS if s[1] > 1024])
+def test_long_rows_within_the_error_of_their_longest_chain(pkg, t, masked, n, v):
+    """Ordinary logits, with less room than a lost chunk of 16 bytes would take on the average.  A thread has at most v / (threads of a row) + 64 values, in two sums, and
+    three roundings for every batch of 16 values or more; a dozen joins; a term is off by (4 + 3 |d|) u with |d| below 10 + log v for those that count."""
+    per, blocks = (4 if t == "f32" else 8), 1
+    while blocks < 8 and n * blocks < 2 * 148 and v >= 256 * per * 4 * blocks:
+        blocks *= 2
+    threads = 256 * blocks if blocks > 1 else 32 if v <= 8192 and n >= 8 * 148 else 128
+    gen = torch.Generator("cuda").manual_seed(n + v)
+    x = torch.randn(n, v, device="cuda", generator=gen).to(TYPES[t])
+    z = x.double()
+    legal = None
+    if masked:
+        legal = torch.rand(n, v, device="cuda", generator=gen) < 0.7
+        z = z.masked_fill(~legal, -np.inf)
+        legal = legal.to(torch.uint8)
+    taken = torch.randint(0, v, (n,), device="cuda", dtype=torch.int32, generator=gen)
+    p, (lp, h, _ta, _tl, st), _keep = forward(pkg, x, t, taken, legal, stats=True)
+    logp = torch.log_softmax(z, 1)
+    pr = logp.exp()
+    chain = v / threads + 64
+    e = (chain / 2 + 3 * chain / 16 + 12 + 4 + 3 * (10 + np.log(v))) * U
+    assert e < per / v / 2
+    want = logp.gather(1, taken.long()[:, None])[:, 0]
+    fine = ~torch.isinf(want)
+    assert torch.equal(~fine, torch.isinf(lp[:n])) and ((lp[:n] - want)[fine].abs() <= e + 4 * U * want[fine].abs()).all()
+    lq = torch.where(pr > 0, logp, 0.0)
+    eh = -(pr * lq).sum(1)
+    assert ((h[:n] - eh).abs() <= e * (2 + eh)).all()
+    gl, gh = torch.randn(n, device="cuda", generator=gen), torch.randn(n, device="cuda", generator=gen) * 0.1
+    g = torch.empty(n, v, dtype=TYPES[t], device="cuda")
+    pkg.policy_logprobs_backward(p, st.data_ptr(), gl.data_ptr(), gh.data_ptr(), g.data_ptr())
+    eg = gl[:, None] * (torch.zeros_like(pr).scatter_(1, taken.long()[:, None], 1.0) - pr) - gh[:, None] * pr * (lq + eh[:, None])
+    if masked:
+        eg[legal == 0] = 0.0
+    tol = pr * (gl.abs()[:, None] + gh.abs()[:, None] * (lq.abs() + eh[:, None] + 1)) * 2 * (e + 8 * U) + eg.abs() * (4 * U + plain.HALF_STEP[t]) + plain.TINY[t]
+    assert ((g.double() - eg).abs() <= tol).all()
