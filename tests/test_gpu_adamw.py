@@ -571,3 +571,44 @@ def test_a_wait_that_runs_out(pkg, bits, max_norm):
     assert opt.get_stats().step == 6
     with pytest.raises(pkg.CudarlError, match="polls"):
         opt.debug_set_copy_wait_polls(-1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_weights_of_a_policy_that_steps_the_arena(pkg, bits):
+    """A policy (a table of logits over the cells, a shared bias) chooses the moves, the calls give its gradient, and its weights and moments after every step are those of
+    the formula in 64 bits, from the weights, moments and gradients before it."""
+    w, h, n = 12, 9, 500
+    world = pkg.VecGridWorld(pkg.make_config(w, h, n, 99, obstacle_kind=pkg.OBST_BERNOULLI, obstacle_p=0.1, goal_mode=pkg.GOAL_SEEDED, num_goals=1, start_mode=pkg.START_RANDOM))
+    gen = torch.Generator("cuda").manual_seed(1)
+    net = Net(pkg, [w * h * 4, 4], bits=bits)
+    for t in net.tensors:
+        for key in ("m", "v", "s1", "s2"):
+            if key in t:
+                t[key].zero_()
+    table, bias = net.tensors[0]["param"].view(w * h, 4), net.tensors[1]["param"]
+    opt = pkg.AdamW(net.list(), state_bits=bits, max_grad_norm=0.002, seed=12)
+    rewards, dones = torch.zeros(n, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda")
+    clipped = 0
+    for step in range(1, 7):
+        x, y, _t = world.get_state()
+        cell = torch.from_numpy(y.astype(np.int64) * w + x).cuda()
+        logits = (table[cell] + bias).contiguous()
+        noise = -torch.log(-torch.log(torch.rand(n, 4, device="cuda", generator=gen).clamp(1e-6, 1 - 1e-6)))
+        taken = (logits + noise).argmax(1).int()
+        torch.cuda.synchronize()
+        assert pkg.load().cudarl_step_actions_device(world.h, taken.data_ptr(), rewards.data_ptr(), dones.data_ptr()) == 0
+        world.synchronize()
+        rows = pkg.PolicyRows(logits.data_ptr(), pkg.F32, n, 4, taken=taken.data_ptr())
+        lp, grad = torch.empty(n, device="cuda"), torch.empty_like(logits)
+        pkg.policy_logprobs(rows, lp.data_ptr())
+        gl, gh = -(rewards - rewards.mean()) / n, torch.full((n,), -0.01 / n, device="cuda")
+        pkg.policy_logprobs_backward(rows, None, gl.data_ptr(), gh.data_ptr(), grad.data_ptr())
+        net.tensors[0]["grad"].view(w * h, 4).zero_().index_add_(0, cell, grad)
+        net.tensors[1]["grad"].copy_(grad.sum(0))
+        before = net.snapshot()
+        norm = np.sqrt(sum((g ** 2).sum() for _w, g, _m, _v in before))
+        clipped += norm > 0.002
+        opt.step(0.05)
+        check(net, before, step, 0.05, min(1.0, float(np.float32(0.002)) / (norm + 1e-6)), seed=12)
+        assert any((t["param"].double().cpu().numpy() != b[0]).any() for t, b in zip(net.tensors, before))
+    assert clipped > 0
