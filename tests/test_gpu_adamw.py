@@ -612,3 +612,72 @@ def test_the_weights_of_a_policy_that_steps_the_arena(pkg, bits):
         check(net, before, step, 0.05, min(1.0, float(np.float32(0.002)) / (norm + 1e-6)), seed=12)
         assert any((t["param"].double().cpu().numpy() != b[0]).any() for t, b in zip(net.tensors, before))
     assert clipped > 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("beta1,beta2,step", [(0.0, 0.0, 0), (0.0, 0.999, 3), (0.9, 0.0, 0), (0.999999, 1 - 1e-9, 0), (0.9, 0.999, 10 ** 15), (0.5, 0.999999, 1 << 62)])
+def test_settings_at_their_ends(pkg, bits, beta1, beta2, step):
+    net = Net(pkg, [300, 5000, 1], "f32", "bf16", False, bits, seed=4)
+    before = net.snapshot()
+    opt = pkg.AdamW(net.list(), state_bits=bits, beta1=beta1, beta2=beta2, seed=2, step=step)
+    opt.step(0.01)
+    check(net, before, step + 1, 0.01, 1.0, 2, beta1, beta2)
+    assert opt.get_stats().step == step + 1
+    before = net.snapshot()
+    opt.step(0.0, grad_scale=0.5)                                            # moments move, weights do not
+    for t, (_w, g, m, v) in zip(net.tensors, before):
+        # the two terms of m' may cancel -- all of a tensor of one value: it is off by three roundings of the terms, whatever is left of them
+        off = 4 * U * (beta1 * np.abs(m) + (1 - beta1) * np.abs(0.5 * g)) + 1e-37
+        em, ev = beta1 * m + (1 - beta1) * 0.5 * g, beta2 * v + (1 - beta2) * 0.25 * g * g
+        if bits == 32:
+            assert (np.abs(t["m"].double().cpu().numpy() - em) <= off).all() and (np.abs(t["v"].double().cpu().numpy() - ev) <= 5 * U * ev + 1e-37).all()
+            continue
+        value = np.concatenate([plain.E4M3, [np.nan], -plain.E4M3, [np.nan]])
+        blocks = [slice(b, b + 256) for b in range(0, len(g), 256)]
+        for key, scale, x, o in (("m", "s1", em, off), ("v", "s2", np.sqrt(ev), 3 * U * np.sqrt(ev))):
+            got, by = t[key].cpu().numpy(), t[scale].double().cpu().numpy()
+            for b, at in enumerate(blocks):
+                high = np.abs(x[at]).max() / 448
+                assert abs(by[b] - high) <= 4 * U * high + o[at].max() / 448
+                assert (np.abs(value[got[at]] * by[b] - x[at]) <= np.maximum(np.abs(x[at]) / 8, by[b] * 2.0 ** -9) * (1 + 8 * U) + o[at]).all()
+    assert all((t["param"].double().cpu().numpy() == b[0]).all() for t, b in zip(net.tensors, before))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_beyond_32_bits(pkg, bits):
+    """2^31 + 777 values: pieces of it on both sides of every power of two, its end, and the rest left at zero."""
+    n = (1 << 31) + 777
+    param, grad = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m, v = (torch.zeros(n, dtype=torch.float32 if bits == 32 else torch.uint8, device="cuda") for _ in range(2))
+    s1, s2 = (torch.zeros((n + 255) // 256, device="cuda") for _ in range(2))
+    windows = [0, (1 << 28) - 256, (1 << 29) - 256, (1 << 30) - 256, (1 << 31) - 512, (1 << 31), n - 521]
+    windows = [w - w % 256 for w in windows]
+    gen = torch.Generator("cuda").manual_seed(1)
+    for w in windows:
+        for x, size in ((param, 1.0), (grad, 1e-2)):                         # (a window may reach into the next)
+            x[w:w + 512] = (torch.randn(min(512, n - w), device="cuda", generator=gen) * size).bfloat16()
+    tensors = [pkg.AdamWTensor(count=n, param=param.data_ptr(), param_type=pkg.BF16, grad=grad.data_ptr(), grad_type=pkg.BF16, moment1=m.data_ptr(), moment2=v.data_ptr(),
+                               scale1=s1.data_ptr(), scale2=s2.data_ptr(), lr_scale=1.0, weight_decay=0.01)]
+    before = [(param[w:w + 512].double().cpu().numpy(), grad[w:w + 512].double().cpu().numpy()) for w in windows]
+    total = sum(float(part.double().square().sum()) for part in grad.split(1 << 28))
+    opt = pkg.AdamW(tensors, state_bits=bits, max_grad_norm=0.1, seed=9)
+    opt.step(0.01)
+    norm = np.sqrt(total)
+    assert abs(opt.get_stats().grad_norm - norm) <= 1e-12 * norm
+    clip = min(1.0, float(np.float32(0.1)) / (norm + 1e-6))
+    for w, (p, g) in zip(windows, before):
+        ep, em, ev = plain.adamw(p, g, np.zeros_like(p), np.zeros_like(p), 1, float(np.float32(0.01)), float(np.float32(0.01)), clip)
+        assert (np.abs(param[w:w + 512].double().cpu().numpy() - ep) <= 1e-6 * 0.01 + plain.HALF_STEP["bf16"] * np.abs(ep) * (1 + 2.0 ** -7)).all()
+        for x, scale, want in ((m, s1, em), (v, s2, np.sqrt(ev))):
+            if bits == 32:
+                want = want if x is m else ev
+                assert (np.abs(x[w:w + 512].double().cpu().numpy() - want) <= 6 * U * np.abs(want) + 1e-37).all()
+            else:
+                value = np.concatenate([plain.E4M3, [np.nan], -plain.E4M3, [np.nan]])
+                by = scale[w // 256:w // 256 + 2].double().cpu().numpy().repeat(256)[:len(want)]
+                got = value[x[w:w + 512].cpu().numpy()] * by
+                assert (np.abs(got - want) <= np.maximum(np.abs(want) / 8, by * 2.0 ** -9) * 1.001).all()
+    for w in windows:                                                        # elsewhere nothing has become anything
+        for x in (param, m, v):
+            x[w:w + 512] = 0
+    assert not any(bool(part.any()) for x in (param, m, v) for part in x.split(1 << 28))

@@ -512,3 +512,48 @@ def test_long_rows_within_the_error_of_their_longest_chain(pkg, t, masked, n, v)
         eg[legal == 0] = 0.0
     tol = pr * (gl.abs()[:, None] + gh.abs()[:, None] * (lq.abs() + eh[:, None] + 1)) * 2 * (e + 8 * U) + eg.abs() * (4 * U + plain.HALF_STEP[t]) + plain.TINY[t]
     assert ((g.double() - eg).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [4, 9, 40, 200, 1500, 9001, 70001])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 1e3, 1e6])
+def test_temperatures_at_their_ends(pkg, t, v, scale):
+    """Rows on both sides of where differences are taken exactly, masks of the lowest value among them."""
+    rng = np.random.default_rng(v)
+    x, taken = some(rng, 12, v)
+    if t != "f16":
+        x[3] *= 1e4
+        x[4] = rng.standard_normal(v) * 1e7
+    x[5] = rng.standard_normal(v) * 1e-4
+    x[6] = float(torch.finfo(TYPES[t]).min); x[6, v // 2] = 1.0
+    x[7] = -np.inf; x[7, 0] = 2.5
+    legal = rng.random((12, v)) < 0.6
+    gl, gh = rng.standard_normal(12) / max(scale, 1), rng.standard_normal(12) * 0.1 / max(scale, 1)
+    for mask in (None, legal):
+        check_forward(pkg, x, t, taken, mask, scale=scale, top=min(v, 5))
+        check_gradient(pkg, x, t, taken, gl, gh, mask, scale=scale)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_the_longest_row(pkg, t):
+    """2^30 actions: one that has all the probability, at the ends and in the middle, and all of them alike (sums of ones are exact up to 2^24 a thread)."""
+    v = 1 << 30
+    x = torch.full((1, v), -np.inf, dtype=TYPES[t], device="cuda")
+    grad = torch.empty(1, v, dtype=TYPES[t], device="cuda")
+    gl = torch.ones(1, device="cuda")
+    for j in (0, 1, (1 << 29) - 1, 1 << 29, v - 5, v - 1):
+        x[0, j] = 1.5
+        taken = torch.tensor([j], dtype=torch.int32, device="cuda")
+        _p, (lp, h, ta, tl, _st), _keep = forward(pkg, x, t, taken, top=1)
+        assert float(lp[0]) == 0.0 and float(h[0]) == 0.0 and int(ta[0]) == j and float(tl[0]) == 0.0
+        other = (j + v // 2) % v
+        p, (lp, _h, _ta, _tl, st), _keep = forward(pkg, x, t, torch.tensor([other], dtype=torch.int32, device="cuda"), stats=True)
+        pkg.policy_logprobs_backward(p, st.data_ptr(), gl.data_ptr(), None, grad.data_ptr())
+        assert float(lp[0]) == -np.inf and float(grad[0, j]) == -1.0 and float(grad[0, other]) == 1.0
+        grad[0, j] = grad[0, other] = 0.0
+        assert not bool(grad.any())
+        x[0, j] = -np.inf
+    x.fill_(0.25)
+    _p, (lp, h, _ta, _tl, _st), _keep = forward(pkg, x, t, torch.tensor([v - 1], dtype=torch.int32, device="cuda"))
+    want = 30 * np.log(2.0)
+    assert abs(float(lp[0]) + want) <= 4 * U * want and abs(float(h[0]) - want) <= 4 * U * want
