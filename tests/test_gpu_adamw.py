@@ -681,3 +681,46 @@ def test_a_tensor_beyond_32_bits(pkg, bits):
         for x in (param, m, v):
             x[w:w + 512] = 0
     assert not any(bool(part.any()) for x in (param, m, v) for part in x.split(1 << 28))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_new_gradients_for_a_captured_step(pkg, bits, offset):
+    """A captured step reads the gradients where they are when it is replayed, aligned as they are then."""
+    net = Net(pkg, [3000, 0, 50], bits=bits)
+    opt = pkg.AdamW(net.list(), state_bits=bits, max_grad_norm=0.5)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step(0.01, stream=torch.cuda.current_stream().cuda_stream)
+    for step in (1, 2):
+        grads = [torch.randn(n + offset, device="cuda")[offset:] for n in net.sizes]
+        opt.set_gradients([x.data_ptr() if x.numel() else None for x in grads])
+        before = [(w, x.double().cpu().numpy(), m, v) for (w, _g, m, v), x in zip(net.snapshot(), grads)]
+        norm = np.sqrt(sum((x ** 2).sum() for _w, x, _m, _v in before))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        check(net, before, step, 0.01, 0.5 / (norm + 1e-6))
+    del g
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_a_gradient_that_is_no_number_without_clipping(pkg, bits, bad):
+    """Its weight becomes NaN; every other takes its step, and outside its block goes on."""
+    net = Net(pkg, [300, 5000], bits=bits)
+    net.tensors[1]["grad"][1025] = bad
+    before = net.snapshot()
+    opt = pkg.AdamW(net.list(), state_bits=bits)
+    opt.step(0.01)
+    weight = net.tensors[1]["param"].double().cpu().numpy()
+    w, g, m, v = before[1]
+    g = g.copy(); g[1025] = 0.0
+    ew, _m, _v = plain.adamw(w, g, m, v, 1, float(np.float32(0.01)), float(np.float32(net.decay)), lr_scale=1.5)
+    keep = np.arange(5000) != 1025
+    assert np.isnan(weight[1025]) and np.isfinite(weight[keep]).all()
+    assert (np.abs(weight - ew)[keep] <= 1e-6 * np.maximum(1, np.abs(ew - w)[keep]) + 2 * U * np.abs(ew)[keep]).all()
+    opt.step(0.01)
+    after = net.tensors[1]["param"].double().cpu().numpy()
+    outside = (np.arange(5000) < 1024) | (np.arange(5000) >= 1280)
+    assert np.isfinite(after[outside]).all() and (after[outside] != weight[outside]).any()
