@@ -5,7 +5,9 @@
 // captured step counts on.
 //
 // What bounds it (B200, kernels alone): with 32-bit moments the memory: 150M values of bf16 weights with masters, 28 bytes each, 695 us = 6.05 TB/s, 92 % of a copy's rate.
-// With 8-bit moments, 16 bytes a value, the instructions: 555 for a warp's 256 values, 141 us for 40M (4.2 TB/s); 200M with the norm 734 us.
+// With 8-bit moments, 16 bytes a value, neither the memory (40M values 137 us: 640 MB in and out = 4.7 TB/s, 585 MB of them past the L2) nor the issue slots (590
+// instructions for a warp's 256 values, 0.60 issued per scheduler and cycle): the warps of a block have their arithmetic at the same time -- for each issue 1.7 warps
+// that could have issued too and 1.3 that wait for an occupied unit -- and then wait for their pieces together.  200M with the norm 740 - 785 us, by the box.
 #include "async_copy.cuh"
 #include "caller_arrays.cuh"
 #include "rules.cuh"
@@ -371,7 +373,7 @@ __device__ __forceinline__ Two root2(Two v) {
 constexpr float INFINITE_ROOT = 36893488147419103232.0f;                     // 2^65
 
 // A block of threads takes a piece, a warp a block of it, a lane eight values.  Every product and sum of the moments is rounded by itself, and the roots and
-// quotients that become codes are correctly rounded (but for one in thousands, off by the last bit): codes do not depend on what a compiler fuses.
+// quotients that become codes are correctly rounded (but for one in thousands, off by the last bit, and roots of less than 2^-100): codes do not depend on what a compiler fuses.
 template <int BITS>
 __global__ void __launch_bounds__(THREADS, RESIDENT) k_adamw(const Tensor* tensors, const Piece* pieces, unsigned n, Control* ctl, const __grid_constant__ Settings s, float lr, float grad_scale) {
     extern __shared__ __align__(128) unsigned char shared_bytes[];

@@ -486,8 +486,11 @@ template <int TYPE> __device__ __forceinline__ void add_chunk(const float (&x)[C
 // A warp a row, the whole row in registers: CHUNKS pieces of 16 bytes a lane, and an end.  What is
 // scalar in a row -- the taken action's logit, logarithm, quotient, addresses, the writes -- is done for up to 32 consecutive rows at a time, a lane each.
 // The alternatives: the `top`-th largest of the lanes' maxima is a bound that `top` values reach; what reaches it is listed, and each of those counts how many
-// are larger.  65,536 x 257 fp32: 26 us (208 instructions a row), with a mask 40 (310), with a mask and 4 alternatives 66 (611): it is the instructions that bound
-// it.  (100,000 x 1000 fp32 with 4 alternatives 119 us, by the kernel for long rows 150; without 76 and 72.  Loading the next row into registers ahead, or having it
+// are larger.  With about 28 of them and more the bound is so low that often more than WARP_KEYS values reach it, and the row is gone through by best_of_all, 32 values at
+// a time: 100,000 x 1000 fp32 with 0 / 4 / 16 / 24 / 28 / 32 alternatives 75 / 117 / 187 / 286 / 717 / 1161 us.
+// 65,536 x 257 fp32: 25 us (209 instructions a row), with a mask 40 (310), with a mask and 4 alternatives 65 (618, 0.63 issued per scheduler and cycle; a warp waits for
+// its row's loads 3.4 and for fixed latencies 3.0 times as long as it issues).  257 values are 64 chunks and an end, and go through a kernel for twice as many: half of
+// its places are empty.  (100,000 x 1000 fp32 with 4 alternatives 119 us, by the kernel for long rows 150; without 76 and 72.  Loading the next row into registers ahead, or having it
 // fetched to L2, made it slower: 92 and 78 us.)
 constexpr int WARP_KEYS = 64, GROUP_KEYS = 128;
 // Blocks on an SM for which the registers suffice.

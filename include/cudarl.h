@@ -264,7 +264,8 @@ typedef struct cudarl_policy_rows {
  * A row in which nothing has any probability (no legal action, or minus infinity in every one): log probability minus
  * infinity, entropy 0.  A row that holds a NaN or plus infinity among its legal logits: NaN, and -1 for its alternatives.
  * Two logits whose difference passes a float's range are infinitely far apart.
- * Sums are held in 32 bits; results do not depend on anything but the row and, in their last bits, on how many there are. */
+ * Sums are held in 32 bits.  The same call gives the same bits every time; equal rows may differ in their last bits with how many rows there are, how a
+ * row's address lies to 16 bytes (rows of more than CUDARL_ACTIONS_WITHOUT_STATS actions), and the device's number of SMs. */
 int cudarl_policy_logprobs(const cudarl_policy_rows* p, float* logprob, float* entropy, float* stats,
                            int32_t top, int32_t* top_actions, float* top_logprobs, void* stream);
 /* grad_logits[r*grad_stride + a] (of the logits' type) = what grad_logprob[rows] and grad_entropy[rows] (either may be NULL =
@@ -279,10 +280,11 @@ int cudarl_policy_logprobs_backward(const cudarl_policy_rows* p, const float* st
  *   w' = w - lr lr_scale (weight_decay w + (m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps))
  * in 32 bits, rounded once to the weights' type (t = 1 for the first step).  With a master the step is that of the master and
  * `param` receives a copy rounded to its type.
+ * Without clipping a gradient that is no finite number makes its weight NaN, and with 8 bits the moments of its block.
  * A v that passes a float's range is infinite: its value stays where it is from then on, but for the decay, until the moments
  * are set anew (with 8 bits its root is kept as 2^65, and its block's scale goes by that).  Clipping keeps v from it.
  * With state_bits = 32 the moments m and v are floats.  With 8, moment1 holds m and moment2 the root of v as e4m3 codes, each
- * block of 256 consecutive values (the last may be shorter) times its scale: the block's largest magnitude / 448.  A code is
+ * block of 256 consecutive values (the last may be shorter) times its scale: the block's largest magnitude times 1 / 448, a float each.  A code is
  * rounded up or down by 16 random bits of the Philox stream of (seed, step, place), so that small changes are not lost on
  * average; a root above zero never becomes 0.  The step itself uses the moments before they are rounded.  Moments (and scales)
  * that are all zero are the start.
@@ -319,14 +321,15 @@ typedef struct cudarl_adamw_stats {
 typedef struct cudarl_adamw cudarl_adamw;
 
 /* The handle keeps the list of the tensors and the step count on the device; the tensors' memory stays the caller's and has
- * to outlive it.  At most 2^34 values, in blocks of 256 counted up for every tensor.  Tensors must not overlap.  One handle's calls are ordered by the caller (one stream, or events). */
+ * to outlive it, and it has to outlive the graphs that a step was captured into.  Creating, destroying and get_stats wait for the device: not while
+ * a stream of it is captured.  At most 2^34 values, in blocks of 256 counted up for every tensor.  Tensors must not overlap.  One handle's calls are ordered by the caller (one stream, or events). */
 int  cudarl_adamw_create(const cudarl_adamw_config* cfg, int32_t count, const cudarl_adamw_tensor* tensors, cudarl_adamw** out);
 /* Waits for the device. */
 void cudarl_adamw_destroy(cudarl_adamw* opt);
 /* One step of all tensors.  The step count is on the device: a captured graph counts on with every replay (lr and grad_scale
  * stay those of the capture). */
 int  cudarl_adamw_step(cudarl_adamw* opt, float lr, float grad_scale, void* stream);
-/* New gradient pointers for the tensors in order (host array of `count` device pointers); not while `stream` is captured. */
+/* New gradient pointers for the tensors in order (host array of `count` device pointers), for captured steps, too; not while `stream` is captured. */
 int  cudarl_adamw_set_gradients(cudarl_adamw* opt, const void* const* grads, void* stream);
 /* Waits for the device.  CUDARL_ERR_DEVICE + CUDARL_DEVERR_COPY_TIMEOUT (statistics filled in) when a wait inside a step ran out: that
  * step is not counted, a part of the tensors may have taken it, and no later step of the handle does anything. */
